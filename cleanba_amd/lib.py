@@ -14,6 +14,8 @@ SO_PATH = os.environ.get("CBM_SO", os.path.join(_HERE, "libcleanba_mi.so"))  # C
 
 NET_NATURE, NET_IMPALA_RESNET = 0, 1
 ALGO_PPO, ALGO_IMPALA = 0, 1
+F32, BF16, F16 = 0, 1, 2              # CBM_F32 ..: types of token logits
+LEARNER_STREAM = 2 ** (8 * C.sizeof(C.c_void_p)) - 1   # CBM_LEARNER_STREAM
 FRAME = 4 * 84 * 84
 
 
@@ -58,6 +60,7 @@ SYMBOLS = [
     "cbm_ipc_close_window", "cbm_ipc_close_all",
     "cbm_host_register", "cbm_host_unregister", "cbm_actor_ship_shard", "cbm_io_sync", "cbm_params_push", "cbm_params_mark_published", "cbm_ctx_abort", "cbm_profile_read_all", "cbm_profile_kernel_name",
     "cbm_comm_native_export", "cbm_comm_native_init", "cbm_comm_backend", "cbm_comm_allreduce_grads", "cbm_comm_overlap_probe",
+    "cbm_top_logits", "cbm_top_logits_workspace", "cbm_distill_loss_grad", "cbm_verify_drafts", "cbm_verify_drafts_workspace",
 ]
 
 COMM_LEARNERS, COMM_WORLD = 0, 1
@@ -128,6 +131,14 @@ def load():
     lib.cbm_synth_env_step_host_to.argtypes = [C.c_uint32, C.c_int32, C.c_int32, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.cbm_comm_load.argtypes = [C.c_char_p]
     lib.cbm_comm_backend.restype = C.c_char_p
+    i32, i64, f32 = C.c_int32, C.c_int64, C.c_float
+    lib.cbm_top_logits_workspace.restype = i64
+    lib.cbm_top_logits_workspace.argtypes = [i32, i32, i32, i32]
+    lib.cbm_top_logits.argtypes = [vp, vp, i32, i32, i32, i64, i32, f32, vp, vp, vp, vp, i64, vp]
+    lib.cbm_distill_loss_grad.argtypes = [vp, vp, i32, i32, i32, i64, vp, vp, i32, vp, vp, f32, vp, vp, i64, vp]
+    lib.cbm_verify_drafts_workspace.restype = i64
+    lib.cbm_verify_drafts_workspace.argtypes = [i32, i32, i32, i32, i32, f32]
+    lib.cbm_verify_drafts.argtypes = [vp, vp, i32, i32, i32, i32, i64, i64, vp, i64, i64, vp, vp, vp, vp, f32, vp, vp, vp, vp, i64, vp]
     _lib = lib
     return lib
 

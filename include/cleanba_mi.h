@@ -282,6 +282,53 @@ int cbm_adam_step(cbm_ctx* ctx, float* p, const float* g, float* m, float* v, in
 int cbm_rmsprop_step(cbm_ctx* ctx, float* p, const float* g, float* nu, int64_t n, float max_norm, float lr,
                      float grad_div);                                                               /* impala:152-188 */
 
+/* ---- token policies: rows of logits over a vocabulary of up to 2^19 tokens, where the functions above hold <= 28 actions.  No reference line:
+ * cleanba's policies end at the action set; these are the same three roles for a policy whose actions are tokens — what a teacher hands over, a policy
+ * loss with its gradient (as cbm_ppo_loss_grad), the ratio of two policies truncated at 1 with the sampling behind it (as cbm_vtrace, cbm_sample).
+ *  - Logits are CBM_F32, CBM_BF16 or CBM_F16, the last axis dense, rows at any stride >= vocab (in elements) and any element-aligned address.  -inf
+ *    masks a token.  Statistics, losses and log-probabilities are fp32 results of fp32 / fp64 sums; gradients have the logits' type, rounded once.
+ *  - ASYNCHRONOUS, unlike the parity functions above: the call enqueues on `stream` (a hipStream_t; NULL is HIP's default stream;
+ *    CBM_LEARNER_STREAM is the context's) and returns.  Nothing is kept between calls and the context is only read, so that any number of threads and
+ *    streams may call at once and calls may be captured into graphs.  The caller's current device is left as it was.
+ *  - The workspace is the caller's: at least cbm_*_workspace(...) bytes (0: may be NULL) at 16-byte alignment, contents irrelevant, not shared by calls
+ *    that may run at the same time.  The *_workspace functions return -1 for sizes that the operator refuses.
+ *  - temperature tau in [1e-4, 1e4]: distributions are softmax(logits / tau). */
+enum { CBM_F32 = 0, CBM_BF16 = 1, CBM_F16 = 2 };
+#define CBM_LEARNER_STREAM ((void*)(intptr_t)-1)
+/* The k (1..256) largest logits of each row, falling, equal ones by rising index (-0 equals +0): idx i32 [rows][k], values f32 [rows][k], and
+ * lse f32 [rows] = log sum_j exp(logits_j / tau).  -inf and NaN are never taken; a slot that stays empty holds idx -1, value -inf.  A row of nothing
+ * but -inf has lse -inf, one with a NaN lse NaN, one with +inf lse +inf. */
+int64_t cbm_top_logits_workspace(int32_t dtype, int32_t rows, int32_t vocab, int32_t k);
+int cbm_top_logits(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, int32_t k, float temperature,
+                   int32_t* idx, float* values, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+/* Distillation from a teacher's top logits: KL(teacher || student) tau^2 per row times row_weight (NULL: 1), and its gradient.
+ *  teacher_idx i32 [rows][k], teacher_logits f32 [rows][k] (k 1..256): the teacher's slots; an index outside [0, vocab) is an empty slot, a token in
+ *    several slots has their probabilities added.
+ *  teacher_lse f32 [rows] or NULL.  NULL: the teacher is softmax over the slots.  Given (at the same tau): slot probabilities are
+ *    exp(logit / tau - lse), what they leave of 1 is one more class, "any other token", in teacher and student alike.
+ *  loss f32 [rows]; dlogits: like logits, rows grad_stride apart, or NULL for the loss alone; it may be logits itself (same pointer and stride).
+ * Loss and gradient of a row are 0 where its weight is 0 (the row is not read), where all its logits are -inf, and where the teacher has no filled slot.
+ * The class of other tokens is left out where the student has no logit above -inf for it.  A student's -inf on a token of the teacher gives loss +inf. */
+int cbm_distill_loss_grad(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, const int32_t* teacher_idx,
+                          const float* teacher_logits, int32_t k, const float* teacher_lse, const float* row_weight, float temperature, float* loss,
+                          void* dlogits, int64_t grad_stride, void* stream);
+/* Verification of drafted tokens against the target's distributions p, from given random numbers; keeps the target's distribution exactly.
+ *  target_logits [batch][drafts+1][vocab], draft_logits [batch][drafts][vocab] or NULL (drafts that were looked up: q is one-hot at the token), strides in
+ *    elements (0 allowed: shared rows); draft_tokens i32 [batch][drafts]; n_draft i32 [batch] or NULL: how many of them count (clamped to [0, drafts]; rows behind are not read);
+ *    u_accept f32 [batch][drafts], u_sample f32 [batch] in [0, 1).
+ *  Draft i is accepted while u_accept_i q_i(x_i) < p_i(x_i).  At the first rejection a one token is drawn from max(p_a - q_a, 0) (from p_a where that is 0
+ *    everywhere), after n acceptances from p_n: the first token whose cumulative weight exceeds u_sample times the whole.
+ *  tokens i32 [batch][drafts+1]: the accepted ones, the drawn one, then -1; accepted i32 [batch]; logprobs f32 [batch][drafts+1] or NULL: log p of each
+ *    token, 0 behind the last.  temperature 0: p is one-hot at the largest logit (lowest index of equal ones), random numbers and draft_logits are not
+ *    looked at and may be NULL, logprobs are 0.
+ *  A token outside [0, vocab) is rejected; so is one whose draft row is no distribution (only -inf, a NaN or +inf), and then the token is drawn from p.
+ *  A target row that is no distribution rejects, and the drawn token is -1.  drafts = 0 samples one token a sequence. */
+int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, float temperature);
+int cbm_verify_drafts(cbm_ctx* ctx, const void* target_logits, int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int64_t target_batch_stride,
+                      int64_t target_pos_stride, const void* draft_logits, int64_t draft_batch_stride, int64_t draft_pos_stride,
+                      const int32_t* draft_tokens, const int32_t* n_draft, const float* u_accept, const float* u_sample, float temperature,
+                      int32_t* tokens, int32_t* accepted, float* logprobs, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- per-kernel HIP-event timing for bench.py's roofline line: brackets every learner-stream launch of
  * the selected implicit-GEMM kernel (ids in DESIGN.md §kernels; -1 = off). */
 #define CBM_PROFILE_ALL (-2)   /* every launch of every id */
