@@ -16,7 +16,8 @@ constexpr int TK_MAX_TOP = 256;         // slots of a row: four a lane of the wa
 constexpr int TK_MAX_DRAFTS = 128;      // one thread a draft in the acceptance step
 
 // ------------------------------------------------------------------------------------------ 16 bytes of logits
-struct Pack { uint32_t w[4]; };
+typedef uint32_t tk_u4 __attribute__((ext_vector_type(4)));
+struct Pack { tk_u4 w; };
 template <int DT> struct Lg { static constexpr int ES = DT == CBM_F32 ? 4 : 2, VEC = 16 / ES; };
 template <int DT> constexpr uint32_t TK_NEG = DT == CBM_F32 ? 0xff800000u : (DT == CBM_BF16 ? 0xff80ff80u : 0xfc00fc00u);   // -inf, twice for 16 bits
 
@@ -28,6 +29,21 @@ template <int DT> __device__ __forceinline__ float tk_get(const Pack& p, int j) 
   const uint32_t w = p.w[j >> 1];
   if constexpr (DT == CBM_BF16) return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
   return (float)__builtin_bit_cast(_Float16, (uint16_t)(j & 1 ? w >> 16 : w & 0xffffu));
+}
+// the largest of a pack's elements, NaN aside
+template <int DT> __device__ __forceinline__ float tk_max(const Pack& p) {
+  if constexpr (DT == CBM_F16) {             // two at a time
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const uint32_t a = p.w[0], b = p.w[1], c = p.w[2], d = p.w[3];   // (bit_cast of a vector's element would take the first)
+    const h2 m = __builtin_elementwise_max(__builtin_elementwise_max(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b)),
+                                           __builtin_elementwise_max(__builtin_bit_cast(h2, c), __builtin_bit_cast(h2, d)));
+    return fmaxf((float)m[0], (float)m[1]);
+  } else {
+    float m = tk_get<DT>(p, 0);
+#pragma unroll
+    for (int j = 1; j < Lg<DT>::VEC; ++j) m = fmaxf(m, tk_get<DT>(p, j));
+    return m;
+  }
 }
 template <int DT> __device__ __forceinline__ float tk_at(const char* row, int e) {   // one element
   if constexpr (DT == CBM_F32) { float f; __builtin_memcpy(&f, row + (size_t)e * 4, 4); return f; }
@@ -50,7 +66,7 @@ template <int DT> __device__ __forceinline__ void tk_set(char* row, int e, float
   else { const _Float16 h = (_Float16)v; __builtin_memcpy(row + (size_t)e * 2, &h, 2); }
 }
 // keeps the compiler from holding the decoded floats of a resident row from one pass over it to the next (twice the registers, spills at 1024 threads)
-__device__ __forceinline__ void tk_redecode(Pack& x) { asm volatile("" : "+v"(x.w[0]), "+v"(x.w[1]), "+v"(x.w[2]), "+v"(x.w[3])); }
+__device__ __forceinline__ void tk_redecode(Pack& x) { asm volatile("" : "+v"(x.w)); }
 // vector `vi` of a row of V elements, -inf behind its end
 template <int DT> __device__ __forceinline__ Pack tk_load(const char* row, int vi, int V) {
   constexpr int VEC = Lg<DT>::VEC, ES = Lg<DT>::ES;
@@ -61,7 +77,7 @@ template <int DT> __device__ __forceinline__ Pack tk_load(const char* row, int v
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       if (e + j < V) {
-        if constexpr (ES == 4) __builtin_memcpy(&x.w[j], row + (size_t)(e + j) * 4, 4);
+        if constexpr (ES == 4) { uint32_t f; __builtin_memcpy(&f, row + (size_t)(e + j) * 4, 4); x.w[j] = f; }
         else {
           uint16_t h; __builtin_memcpy(&h, row + (size_t)(e + j) * 2, 2);
           x.w[j >> 1] = j & 1 ? (x.w[j >> 1] & 0xffffu) | ((uint32_t)h << 16) : (x.w[j >> 1] & 0xffff0000u) | h;
@@ -74,6 +90,26 @@ template <int DT> __device__ __forceinline__ Pack tk_load(const char* row, int v
 
 __device__ __forceinline__ float tk_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float tk_base(float m) { return m == -INFINITY ? 0.0f : m; }   // what a maximum of -inf is replaced by: exp2(-inf - 0) = 0, not NaN
+
+// sum of 2^((z - b) c) over a pack, b >= every z.  One fma an element: 2^(z c - bc) with bc = fl(b c), what bc was rounded by goes into `fix` once a thread;
+// a maximum so large that b c might overflow takes the difference first.
+struct ExpSum {
+  float b, c, bc, fix;
+  bool big;
+  __device__ __forceinline__ ExpSum(float base, float c_) : b(base), c(c_), bc(base * c_), big(fabsf(base) > 1e30f) { fix = big ? 1.0f : tk_exp2(-fmaf(base, c_, -bc)); }
+  template <int DT> __device__ __forceinline__ float usual(const Pack& x) const {
+    float p = 0.0f;
+#pragma unroll
+    for (int j = 0; j < Lg<DT>::VEC; ++j) p += tk_exp2(fmaf(tk_get<DT>(x, j), c, -bc));
+    return p;
+  }
+  template <int DT> __device__ __forceinline__ float large(const Pack& x) const {
+    float p = 0.0f;
+#pragma unroll
+    for (int j = 0; j < Lg<DT>::VEC; ++j) p += tk_exp2((tk_get<DT>(x, j) - b) * c);
+    return p;
+  }
+};
 
 // ------------------------------------------------------------------------------------------ reductions
 template <class Tp> __device__ __forceinline__ Tp wave_sum(Tp v) { for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64); return v; }
@@ -330,16 +366,17 @@ void distill_dispatch(const DistillArgs& a, int rows, hipStream_t st) {
 
 // ------------------------------------------------------------------------------------------ the K largest logits of a row
 // Keys: (order of the fp32 value, 19 bits of 2^19 - 1 - index): unique, and their order is "larger value first, equal values by rising index".
-// A block streams its row (or its share of one: few rows are split and joined) in chunks of 16 elements a thread, with the running maximum and
-// sum a thread for the log-sum-exp, and appends what beats the threshold to a buffer in LDS.  The threshold comes from the chunk itself: the
-// K-th largest of the threads' maxima has K elements at or above it, and with T >= 4 K threads few more (1.15 K of random data, at most 16 K
-// of any, which is what the buffer has room for).  An element that only equals the threshold comes behind K others and is left out.
-// A full buffer is cut by the same rule on its own keys, until each thread holds one and the cut is exact.
+// A block streams its row (or its share of one: few rows are split and joined) in chunks of EPT elements a thread, with the running maximum and
+// sum a thread for the log-sum-exp, and appends what is above a bar to a buffer in LDS.  The first bar comes from the first chunk: the K-th largest
+// of the threads' maxima has K elements at or above it, and with T >= 4 K threads few more (1.2 K of random data).  After the 2nd, 4th, 8th .. chunk the
+// K-th largest key of the buffer raises it, so that a row of n chunks appends about K (1 + log2 n) keys.  An element that only equals the bar comes
+// behind K others and is left out.  Should the buffer overflow all the same (rising rows), the lanes that found no room wait while it is cut to T keys,
+// and a chunk that alone would fill it is held to the exact K-th of its threads' maxima: K threads, EPT K keys, the room there is.
 struct TopArgs {
   const char* logits; int64_t ld;
   int32_t* idx; float* val; float* lse;
   uint64_t* ws_keys; MS* ws_ms;              // with nsplit > 1: [row][split][K] and [row][split]
-  int V, K, nsplit, cap;                     // cap = 16 K + T keys
+  int V, K, nsplit, cap, rows;               // cap = EPT K + T keys
   float c;
   double inv_tau;
 };
@@ -348,51 +385,59 @@ __device__ __forceinline__ uint32_t top_order(float v) {   // unsigned order of 
   return u ^ (uint32_t)(((int32_t)u >> 31) | (int32_t)0x80000000);
 }
 __device__ __forceinline__ float top_value(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+__device__ __forceinline__ float top_below(uint32_t o) { return o == 0x80000000u ? __uint_as_float(0x80000001u) : top_value(o - 1); }   // the next smaller number (of 0: of -0 too)
 __device__ __forceinline__ uint64_t top_key(float v, int e) { return ((uint64_t)top_order(v) << 19) | (uint32_t)(TK_MAX_VOCAB - 1 - e); }
+__device__ __forceinline__ int top_index(uint64_t key) { return TK_MAX_VOCAB - 1 - (int)(key & (TK_MAX_VOCAB - 1)); }
+__device__ __forceinline__ uint32_t top_order_of(uint64_t key) { return (uint32_t)(key >> 19); }
 constexpr int TOP_KEY_BITS = 51;
 
-// the largest bound that K of the block's T keys (0: none) reach, or 0 where fewer are there.  The first wave's work.
-template <int T> __device__ uint64_t top_bound(uint64_t key, int K, uint64_t* sk, uint64_t* sbound) {
-  sk[threadIdx.x] = key;
+// the largest bound that K of the block's T numbers (0: none) reach, or 0 where fewer are there; the first wave's work.  With slack, any bound that K .. K + slack
+// of them reach: a third of the steps.
+template <int T, class Num> __device__ Num top_bound(Num mine, int bits, int K, int slack, Num* all, Num* sbound) {
+  all[threadIdx.x] = mine;
   __syncthreads();
   if (threadIdx.x < 64) {
-    uint64_t k[T / 64];
+    Num k[T / 64];
 #pragma unroll
-    for (int i = 0; i < T / 64; ++i) k[i] = sk[i * 64 + threadIdx.x];
-    uint64_t b = 0;
-    for (int bit = TOP_KEY_BITS - 1; bit >= 0; --bit) {
-      const uint64_t cand = b | (1ull << bit);
+    for (int i = 0; i < T / 64; ++i) k[i] = all[i * 64 + threadIdx.x];
+    Num b = 0;
+    for (int bit = bits - 1; bit >= 0; --bit) {
+      const Num cand = b | ((Num)1 << bit);
       int n = 0;
 #pragma unroll
       for (int i = 0; i < T / 64; ++i) n += __popcll(__ballot(k[i] >= cand));
-      if (n >= K) b = cand;
-      if (n == K) break;
+      if (n >= K) { b = cand; if (n <= K + slack) break; }
     }
     if (threadIdx.x == 0) *sbound = b;
   }
   __syncthreads();
-  const uint64_t b = *sbound;
+  const Num b = *sbound;
   __syncthreads();
   return b;
 }
-// the buffer's n <= 5 T keys cut to at most T, the K largest among them; returns their number and raises the bar
-template <int T> __device__ int top_cut(uint64_t* buf, int n, int K, float* bar, int* sfill, uint64_t* sk, uint64_t* sbound) {
-  constexpr int MOST = 5;   // cap = 16 K + T keys, K <= T / 4
-  while (n > T) {
+template <int T> struct TopShared { uint64_t all[T]; uint64_t bound; int fill; };
+// the buffer's n keys (0: none) cut to the K largest and at most `most` (K <= most <= T) in all; returns their number and raises the bar
+template <int T, int EPT> __device__ int top_cut(uint64_t* buf, int n, int K, int most, float* bar, TopShared<T>& sh) {
+  constexpr int MOST = EPT / 4 + 1;          // n <= cap = EPT K + T, K <= T / 4
+  bool exact = false;
+  while (n > most) {
     uint64_t k[MOST], best = 0;
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
       k[i] = i * T + (int)threadIdx.x < n ? buf[i * T + threadIdx.x] : 0;
       best = k[i] > best ? k[i] : best;
     }
-    const uint64_t bound = top_bound<T>(best, K, sk, sbound);   // (its barriers stand between the reads above and the writes below)
-    if (bound) *bar = fmaxf(*bar, top_value((uint32_t)(bound >> 19)));
-    if (threadIdx.x == 0) *sfill = 0;
+    uint64_t bound;                          // (its barriers stand between the reads above and the writes below)
+    if (exact) bound = top_bound<T, uint64_t>(best, TOP_KEY_BITS, K, 0, sh.all, &sh.bound);
+    else bound = (uint64_t)top_bound<T, uint32_t>(top_order_of(best), 32, K, K / 4, (uint32_t*)sh.all, (uint32_t*)&sh.bound) << 19;
+    if (bound) *bar = fmaxf(*bar, top_value(top_order_of(bound)));
+    if (threadIdx.x == 0) sh.fill = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < MOST; ++i) if (k[i] != 0 && k[i] >= bound) buf[atomicAdd(sfill, 1)] = k[i];
+    for (int i = 0; i < MOST; ++i) if (k[i] != 0 && k[i] >= bound) buf[atomicAdd(&sh.fill, 1)] = k[i];
     __syncthreads();
-    n = *sfill;
+    n = sh.fill;
+    exact = true;                            // (equal values may have kept too many: the next turn tells them apart by their indices)
     __syncthreads();
   }
   return n;
@@ -402,10 +447,11 @@ template <int T> __device__ void top_write(const uint64_t* buf, int n, int K, in
   if ((int)threadIdx.x < n) {
     const uint64_t mine = buf[threadIdx.x];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += buf[j] > mine;
     if (rank < K) {
       if (keys) keys[rank] = mine;
-      else { idx[rank] = TK_MAX_VOCAB - 1 - (int)(mine & (TK_MAX_VOCAB - 1)); val[rank] = top_value((uint32_t)(mine >> 19)); }
+      else { idx[rank] = top_index(mine); val[rank] = top_value(top_order_of(mine)); }
     }
   }
   for (int k = n + (int)threadIdx.x; k < K; k += T) {
@@ -419,105 +465,151 @@ __device__ __forceinline__ float top_lse(MS ms, double inv_tau) {
   return (float)((double)tk_base(ms.m) * inv_tau + log(ms.s));
 }
 
-template <int DT, int T>
+// a chunk's vectors of a thread; -inf behind the row's last whole vector
+template <int DT, int T, int U> __device__ __forceinline__ void top_chunk(Pack (&y)[U], const char* row, int ch, int nfull) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) y[u] = tk_load16(row + (size_t)min((ch * U + u) * T + (int)threadIdx.x, nfull - 1) * 16);
+  if ((ch + 1) * T * U > nfull) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) if ((ch * U + u) * T + (int)threadIdx.x >= nfull) y[u] = tk_neg<DT>();
+  }
+}
+template <int DT, int T, int EPT, int G>
 __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
-  constexpr int VEC = Lg<DT>::VEC, U = 16 / VEC;
+  constexpr int VEC = Lg<DT>::VEC, U = EPT / VEC;
   extern __shared__ uint64_t buf[];          // [cap]
-  __shared__ uint64_t sk[T];
-  __shared__ uint64_t sbound;
+  __shared__ TopShared<T> sh;
   __shared__ MS red[T / 64];
-  __shared__ int scount[3], sfill;
+  __shared__ int sfull[3];                   // whether a chunk's elements found no room: one a pass, in turn
   const int tid = threadIdx.x, V = a.V, K = a.K;
   const int64_t r = blockIdx.x / (uint32_t)a.nsplit;
   const int split = (int)(blockIdx.x - r * a.nsplit);
   const char* row = a.logits + r * a.ld;
-  const int nvec = (V + VEC - 1) / VEC, nchunk = (nvec + T * U - 1) / (T * U);
+  const int nfull = V / VEC, rem = V - nfull * VEC, nchunk = (nfull + T * U - 1) / (T * U);   // (V > 64: there are whole vectors)
   const int c0 = (int)((int64_t)nchunk * split / a.nsplit), c1 = (int)((int64_t)nchunk * (split + 1) / a.nsplit);
-  if (tid < 3) scount[tid] = 0;
-  if (tid == 3) sfill = 0;
-  __syncthreads();
+  const float extra = split == a.nsplit - 1 && tid < rem ? tk_at<DT>(row, nfull * VEC + tid) : -INFINITY;   // the row's last few elements, one a thread
+  Pack x[G][U];                              // G chunks at a time: one bar, one maximum, one rescaling for all; each chunk's registers take the next group's as it is done
+#pragma unroll
+  for (int g = 0; g < G; ++g) top_chunk<DT, T, U>(x[g], row, c0 + g < c1 ? c0 + g : nchunk, nfull);
+  if (tid == 0) sh.fill = 0;
+  if (tid < 3) sfull[tid] = 0;
   float bar = -INFINITY;                     // an element has to be above it
-  int fill = 0;                              // keys in the buffer
-  float m = -INFINITY, s = 0.0f;
-  Pack x[U], y[U];
+  float m = extra, s = extra == -INFINITY ? 0.0f : tk_exp2(extra - extra);   // 1, or NaN
+  int turn = 0, done = 0;
+  __syncthreads();
+  for (int c = c0; c < c1; c += G) {
+    float vm[G][U], cm = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < U; ++u) y[u] = c0 < c1 ? tk_load<DT>(row, (c0 * U + u) * T + tid, V) : tk_neg<DT>();
-  int turn = 0;                              // which of the three counters
-  for (int ch = c0; ch < c1; ++ch) {
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      x[u] = y[u];
-      if (ch + 1 < c1) y[u] = tk_load<DT>(row, ((ch + 1) * U + u) * T + tid, V);
-    }
-    float cm = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) cm = fmaxf(cm, tk_get<DT>(x[u], j));
-    const float nm = fmaxf(m, cm), b = tk_base(nm);
+      for (int u = 0; u < U; ++u) {
+        vm[g][u] = tk_max<DT>(x[g][u]);
+        cm = fmaxf(cm, vm[g][u]);
+        tk_redecode(x[g][u]);
+      }
+    const float nm = fmaxf(m, cm);
+    const ExpSum es(tk_base(nm), a.c);
     float p = 0.0f;
+    if (!es.big) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) p += tk_exp2((tk_get<DT>(x[u], j) - b) * a.c);
-    s = s * tk_exp2((m - b) * a.c) + p;
+        for (int u = 0; u < U; ++u) { p += es.usual<DT>(x[g][u]); tk_redecode(x[g][u]); }
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int u = 0; u < U; ++u) { p += es.large<DT>(x[g][u]); tk_redecode(x[g][u]); }
+    }
+    s = s * tk_exp2((m - es.b) * a.c) + p * es.fix;
     m = nm;
-    // how many of the chunk's elements are above the bar
-    const auto above = [&] {
-      int n = 0;
-      if (cm > bar) {
+    float over = bar;                        // what an element of this group has to be above: just below the bar while equal ones may come before those that made it
+    if (c == c0) {
+      const uint32_t o = top_bound<T, uint32_t>(cm > -INFINITY ? top_order(cm) : 0u, 32, K, K / 4, (uint32_t*)sh.all, (uint32_t*)&sh.bound);
+      if (o) { bar = top_value(o); over = top_below(o); }
+    }
+    uint32_t wait[G];                        // the thread's elements that are above, a bit each
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+    for (int g = 0; g < G; ++g) {
+      wait[g] = 0;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) n += tk_get<DT>(x[u], j) > bar;
-        atomicAdd(&scount[turn], n);
+      for (int u = 0; u < U; ++u) {
+        if (!(vm[g][u] > over)) continue;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int q = VEC - 1; q >= 0; --q) bits = bits + bits + (tk_get<DT>(x[g][u], q) > over ? 1u : 0u);
+        wait[g] |= bits << (u * VEC);
       }
-      __syncthreads();
-      const int t = scount[turn];
-      if (tid == 0) scount[turn == 0 ? 2 : turn - 1] = 0;   // the counter of the turn before: nobody reads it any more, and two barriers pass until it counts again
-      turn = turn == 2 ? 0 : turn + 1;
-      return t;
+      if (c + G < c1) top_chunk<DT, T, U>(x[g], row, c + G + g < c1 ? c + G + g : nchunk, nfull);
+    }
+    // appends those that reach the bound; what finds no room stays.  (Elements again from memory: an indexed register would cost more, and hits are few.)
+    const auto append = [&](uint32_t waits, int ch, uint64_t bound) {
+      uint32_t left = 0;
+      for (uint32_t w = waits; w; w &= w - 1) {
+        const int q = __builtin_ctz(w), e = ((ch * U + q / VEC) * T + tid) * VEC + q % VEC;
+        const float z = tk_at<DT>(row, e);
+        const uint64_t k = top_key(z, e);
+        if (z > over && k >= bound) {
+          const int at = atomicAdd(&sh.fill, 1);
+          if (at < a.cap) buf[at] = k;
+          else left |= 1u << q;
+        }
+      }
+      return left;
     };
-    int n = above();
-    if (n == 0) continue;
-    uint64_t bound = 0;
-    if (fill + n > a.cap) {
-      if (fill > T) {
-        fill = top_cut<T>(buf, fill, K, &bar, &sfill, sk, &sbound);
-        n = above();
-      }
-      if (fill + n > a.cap) {
-        uint64_t best = 0;
-        if (cm > bar) {
+    bool any = false;
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = VEC - 1; j >= 0; --j) {
-              const float z = tk_get<DT>(x[u], j);
-              if (z == cm) { const uint64_t k = top_key(z, ((ch * U + u) * T + tid) * VEC + j); best = k > best ? k : best; }
-            }
-        }
-        bound = top_bound<T>(best, K, sk, &sbound);
-      }
+    for (int g = 0; g < G; ++g) {
+      if (wait[g]) wait[g] = append(wait[g], c + g, 0);
+      any |= wait[g] != 0;
     }
-    if (cm > bar) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float z = tk_get<DT>(x[u], j);
-          if (z > bar) {
-            const uint64_t k = top_key(z, ((ch * U + u) * T + tid) * VEC + j);
-            if (k >= bound) { const int at = atomicAdd(&sfill, 1); if (at < a.cap) buf[at] = k; }
-          }
-        }
-    }
-    if (bound) bar = fmaxf(bar, top_value((uint32_t)(bound >> 19)));
+    if (any) sfull[turn] = 1;
     __syncthreads();
-    fill = sfill;
+    const bool full = sfull[turn] != 0;      // (the same for every thread: this turn's flag is written before the barrier only)
+    if (tid == 0) sfull[turn == 0 ? 2 : turn - 1] = 0;   // the turn before: read by all before this barrier, written again behind the next but one
+    turn = turn == 2 ? 0 : turn + 1;
+    if (full) {                              // chunk by chunk: cut, then what reaches the exact K-th of the waiting maxima fits
+#pragma unroll 1
+      for (int g = 0; g < G; ++g) {
+        uint32_t w = wait[0];
+#pragma unroll
+        for (int q = 1; q < G; ++q) w = q == g ? wait[q] : w;
+        const int fill = min(sh.fill, a.cap);
+        __syncthreads();
+        top_cut<T, EPT>(buf, fill, K, T, &bar, sh);
+        over = top_below(top_order(bar));
+        uint64_t best = 0;
+        for (uint32_t v = w; v; v &= v - 1) {
+          const int q = __builtin_ctz(v), e = (((c + g) * U + q / VEC) * T + tid) * VEC + q % VEC;
+          const float z = tk_at<DT>(row, e);
+          const uint64_t k = top_key(z, e);
+          if (z > over && k > best) best = k;
+        }
+        const uint64_t bound = top_bound<T, uint64_t>(best, TOP_KEY_BITS, K, 0, sh.all, &sh.bound);   // (0: fewer than K threads wait, all they hold fits)
+        append(w, c + g, bound);
+        __syncthreads();
+      }
+    }
+    ++done;
+    if (done > 1 && (done & (done - 1)) == 0 && c + G < c1) {   // what the buffer says about the bar
+      const int fill = sh.fill;              // (no appends before top_bound's barriers)
+      uint32_t o = tid < fill ? top_order_of(buf[tid]) : 0u;
+      if (tid + T < fill) { const uint32_t o2 = top_order_of(buf[tid + T]); o = o2 > o ? o2 : o; }
+      o = top_bound<T, uint32_t>(o, 32, K, K / 4, (uint32_t*)sh.all, (uint32_t*)&sh.bound);
+      if (o) bar = fmaxf(bar, top_value(o));
+    }
   }
   __syncthreads();
-  fill = top_cut<T>(buf, fill, K, &bar, &sfill, sk, &sbound);
+  int fill = sh.fill;
+  __syncthreads();
+  fill = top_cut<T, EPT>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
+  if (rem && split == a.nsplit - 1) {        // (cap has room for EPT K more than T)
+    if (extra > bar) buf[atomicAdd(&sh.fill, 1)] = top_key(extra, nfull * VEC + tid);
+    __syncthreads();
+    fill = sh.fill;
+    __syncthreads();
+    fill = top_cut<T, EPT>(buf, fill, K, T, &bar, sh);
+  }
   const MS ms = block_lse<T>(m, s, a.c, red);
   if (a.nsplit > 1) {
     top_write<T>(buf, fill, K, nullptr, nullptr, a.ws_keys + (r * a.nsplit + split) * K);
@@ -528,351 +620,502 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
   }
 }
 // the splits of a row: their keys are one more buffer to cut
-template <int T>
+template <int T, int EPT>
 __global__ __launch_bounds__(T) void top_join_kernel(TopArgs a) {
   extern __shared__ uint64_t buf[];
-  __shared__ uint64_t sk[T];
-  __shared__ uint64_t sbound;
-  __shared__ int sfill;
-  const int tid = threadIdx.x, K = a.K;
+  __shared__ TopShared<T> sh;
+  const int tid = threadIdx.x, K = a.K, n = a.nsplit * K;
   const int64_t r = blockIdx.x;
-  if (tid == 0) sfill = 0;
+  if (tid == 0) sh.fill = 0;
   __syncthreads();
-  for (int i = tid; i < a.nsplit * K; i += T) {
-    const uint64_t k = a.ws_keys[r * a.nsplit * K + i];
-    if (k) buf[atomicAdd(&sfill, 1)] = k;
+  for (int i = tid; i < n; i += T) { const uint64_t k = a.ws_keys[r * n + i]; if (k) buf[atomicAdd(&sh.fill, 1)] = k; }
+  if (tid < 64) {
+    MS ms = tid < a.nsplit ? a.ws_ms[r * a.nsplit + tid] : MS{-INFINITY, 0.0};
+    const float M = wave_max(ms.m);
+    const double S = wave_sum(ms.s * (double)tk_exp2((ms.m - tk_base(M)) * a.c));
+    if (tid == 0) a.lse[r] = top_lse(MS{M, S}, a.inv_tau);
   }
   __syncthreads();
-  int fill = sfill;
   float bar = -INFINITY;
+  int fill = sh.fill;
   __syncthreads();
-  fill = top_cut<T>(buf, fill, K, &bar, &sfill, sk, &sbound);
+  fill = top_cut<T, EPT>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
   top_write<T>(buf, fill, K, a.idx + r * K, a.val + r * K, nullptr);
-  if (tid == 0) {
-    MS ms = a.ws_ms[r * a.nsplit];
-    for (int i = 1; i < a.nsplit; ++i) {
-      const MS o = a.ws_ms[r * a.nsplit + i];
-      const float M = fmaxf(ms.m, o.m), B = tk_base(M);
-      ms.s = ms.s * (double)tk_exp2((ms.m - B) * a.c) + o.s * (double)tk_exp2((o.m - B) * a.c);
-      ms.m = M;
-    }
-    a.lse[r] = top_lse(ms, a.inv_tau);
-  }
 }
+
+// A vocabulary of a few tokens (an action set): one token a lane, G lanes a row, 64 / G rows a wave; a token's place is the number of tokens before it.
+template <int DT, int G>
+__global__ __launch_bounds__(256) void top_small_kernel(TopArgs a) {
+  const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const int e = threadIdx.x % G, V = a.V, K = a.K;
+  if (r >= a.rows) return;
+  const float z = e < V ? tk_at<DT>(a.logits + r * a.ld, e) : -INFINITY;
+  float m = z;
+  for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, G));
+  float s = tk_exp2((z - tk_base(m)) * a.c);
+  for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, G);
+  const uint32_t mine = z > -INFINITY ? top_order(z) : 0u;   // (a NaN is not above -inf)
+  int rank = 0, n = 0;
+  for (int j = 0; j < V; ++j) {
+    const uint32_t o = (uint32_t)__shfl((int)mine, j, G);
+    rank += o > mine || (o == mine && j < e);
+    n += o != 0;
+  }
+  if (mine && rank < K) { a.idx[r * K + rank] = e; a.val[r * K + rank] = z + 0.0f; }
+  for (int k = n + e; k < K; k += G) { a.idx[r * K + k] = -1; a.val[r * K + k] = -INFINITY; }
+  if (e == 0) a.lse[r] = top_lse(MS{m, (double)s}, a.inv_tau);
+}
+
 struct TopPlan { int threads, nsplit, cap; size_t lds, ws; };
-TopPlan top_plan(int rows, int V, int K, int es) {
-  TopPlan p;
+int top_ept(int threads) { return threads == 256 ? 32 : 16; }
+TopPlan top_plan(int rows, int V, int K) {
+  TopPlan p = {};
+  p.nsplit = 1;
+  if (V <= 64) return p;                     // top_small_kernel
   p.threads = K <= 16 && V <= 1024 ? 64 : (K <= 64 ? 256 : (K <= 128 ? 512 : 1024));   // T >= 4 K
-  p.cap = 16 * K + p.threads;
-  const int chunk = p.threads * 16, nchunk = (V + chunk - 1) / chunk;
+  p.cap = top_ept(p.threads) * K + p.threads;
+  const int chunk = p.threads * top_ept(p.threads), nchunk = (V + chunk - 1) / chunk;
   // few rows: split until there are about 512 blocks; the join holds nsplit K <= cap keys
   int n = rows >= 512 ? 1 : (512 + rows - 1) / rows;
   n = n < nchunk ? n : nchunk;
-  n = n < p.cap / K ? n : p.cap / K;
   p.nsplit = n < 16 ? n : 16;
   p.lds = (size_t)p.cap * 8;
   p.ws = p.nsplit > 1 ? (size_t)rows * p.nsplit * ((size_t)K * 8 + sizeof(MS)) : 0;
-  (void)es;
   return p;
 }
-template <int DT, int T> void top_launch(const TopArgs& a, int rows, const TopPlan& p, hipStream_t st) {
-  hipLaunchKernelGGL((top_kernel<DT, T>), dim3((uint32_t)rows * p.nsplit), dim3(T), p.lds, st, a);
-  if (p.nsplit > 1) hipLaunchKernelGGL(top_join_kernel<T>, dim3(rows), dim3(T), p.lds, st, a);
+template <int DT, int T, int EPT, int G> void top_launch(const TopArgs& a, const TopPlan& p, hipStream_t st) {
+  hipLaunchKernelGGL((top_kernel<DT, T, EPT, G>), dim3((uint32_t)a.rows * p.nsplit), dim3(T), p.lds, st, a);
+  if (p.nsplit > 1) hipLaunchKernelGGL((top_join_kernel<T, EPT>), dim3(a.rows), dim3(T), p.lds, st, a);
 }
-template <int DT> void top_dispatch(const TopArgs& a, int rows, const TopPlan& p, hipStream_t st) {
-  if (p.threads == 64) top_launch<DT, 64>(a, rows, p, st);
-  else if (p.threads == 256) top_launch<DT, 256>(a, rows, p, st);
-  else if (p.threads == 512) top_launch<DT, 512>(a, rows, p, st);
-  else top_launch<DT, 1024>(a, rows, p, st);
+template <int DT, int G> void top_launch_small(const TopArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((top_small_kernel<DT, G>), dim3((uint32_t)(((int64_t)a.rows * G + 255) / 256)), dim3(256), 0, st, a);
+}
+template <int DT> void top_dispatch(const TopArgs& a, const TopPlan& p, hipStream_t st) {
+  if (a.V <= 16) top_launch_small<DT, 16>(a, st);
+  else if (a.V <= 32) top_launch_small<DT, 32>(a, st);
+  else if (a.V <= 64) top_launch_small<DT, 64>(a, st);
+  else if (p.threads == 64) top_launch<DT, 64, 16, 1>(a, p, st);
+  else if (p.threads == 256) top_launch<DT, 256, 32, Lg<DT>::VEC / 4>(a, p, st);
+  else if (p.threads == 512) top_launch<DT, 512, 16, 4>(a, p, st);
+  else top_launch<DT, 1024, 16, 2>(a, p, st);
 }
 
 // ------------------------------------------------------------------------------------------ drafted tokens against the target
 // p_i = softmax(target row i / tau), q_i = softmax(draft row i / tau), or one-hot at the drafted token where there are no draft logits.
 //   accepted while u_i q_i(x_i) < p_i(x_i), i < n;  at the first rejection a the next token is drawn from max(p_a - q_a, 0) (from p_a where that has
 //   no mass), after n acceptances from p_n: the first token whose cumulative weight exceeds u_s times the whole.
-// An acceptance compares two numbers; a drawn token lies between two neighbours of a cumulative sum over the whole vocabulary, so that the row the token
-// is drawn from is summed in fp64 throughout (exps too), chunk by chunk of 4096 tokens, and the statistics of all other rows with fp32 exps.
-//   verify_stats_kernel   (maximum, sum) of the rows of every drafted position, split over blocks
-//   verify_sums_kernel    acceptance (each block of a sequence for itself), then the chunks' fp64 sums of the row that the token is drawn from
-//   verify_rest_kernel    the chunks' sums of max(p - q, 0), where the sequence has a rejection and a draft distribution
-//   verify_pick_kernel    the chunk, then the token inside it
-constexpr int VF_T = 256, VF_CHUNK = 4096;   // 16 tokens a thread
+// The drawn token lies between two neighbours of a cumulative sum over the whole vocabulary: sums that are off by 1e-7 would move one token in a few
+// hundred, so that the row it is drawn from is summed in fp64, exponentials too.  They are 2^(z C - E), C = log2(e) / tau, with a whole number E a chunk of
+// 2048 tokens (the maximum's exponent, rounded up): sums of different chunks are brought together by exact shifts of the exponent.  An acceptance compares
+// two numbers, and sums of fp32 exponentials do for it.
+// Small calls, two kernels (launches are what they cost):
+//   verify_sums_kernel<true>   fp64 sums of each chunk of each row that a sequence may need (a wave a chunk), and of the chunks of a block together
+//   verify_pick_kernel<true>   acceptance, by every block of a sequence for itself; where it ends in a rejection with a draft distribution the chunks' sums of
+//                              max(p - q, 0), and the sequence's last block to finish draws the token; elsewhere its first block draws from the sums there are
+// Large calls, three kernels (an fp64 exponential is 20 instructions, an fp32 one with its sum 6, and but two rows a sequence need the former):
+//   verify_stats_kernel        (maximum, sum) in fp32 of the drafted positions' rows
+//   verify_sums_kernel<false>  acceptance, and the fp64 sums of the one or two rows that the token is drawn from
+//   verify_pick_kernel<false>  the rest as above
+constexpr int VF_T = 256, VF_WAVES = VF_T / 64, VF_CHUNK = 2048;   // 32 tokens a lane: what a chunk costs beside its exps (reductions) is shared by that many
+struct VfSum { double e, s; };               // s 2^e; nothing: s = 0, e = -inf; a NaN among the logits: s NaN; +inf: e = +inf
 struct VerifyArgs {
   const char* target; int64_t tb, tp;        // bytes from sequence to sequence, from position to position
   const char* draft; int64_t db, dp;         // null: no draft distribution
   const int32_t* tokens; const int32_t* n_draft; const float* u_accept; const float* u_sample;
   int32_t* out; int32_t* accepted; float* logprobs;
-  MS* stats;                                 // [position][sequence][target, draft][split]
-  struct VfSum* sums;                        // [sequence][chunk]
-  double* rest;                              // [sequence][chunk]
-  int B, K, V, nsplit, nchunk;
+  MS* stats;                                 // [row][split] in fp32; rows: [sequence][drafts] of the target, then of the draft
+  VfSum* sums;                               // [row][chunk]; rows: [sequence][drafts + 1] of the target, then [sequence][drafts] of the draft; after an acceptance in
+                                             // fp32: [sequence] of the target, then of the draft, the row that was stopped at
+  VfSum* parts;                              // [row][split]: a block's chunks together
+  double* rest;                              // [sequence][chunk]: sums of max(p - q, 0)
+  uint32_t* done;                            // [sequence]: blocks that have finished; cleared by the first kernel for the second
+  int B, K, V, nchunk, nstat, nsplit, npick; // splits of a row in fp32 and in fp64, blocks a sequence in the last kernel
   float c;
-  double inv_tau;
+  double C;
 };
-struct VfSum { double p, q; float mp, mq; }; // sums of exp((z - m) / tau) over a chunk, and its maxima; without draft logits q is what the rejected token alone adds to p
 __device__ __forceinline__ int vf_drafts(const VerifyArgs& a, int b) {
   const int n = a.n_draft ? a.n_draft[b] : a.K;
   return n < 0 ? 0 : (n > a.K ? a.K : n);
 }
+// 2^(z C - E), at most about 1: 32 (z C - E) = 32 k + i + r, |r| <= 1/2: 2^k * table[i] * 2^(r/32), the last one by its series to the fourth power (off by
+// 1.2e-12 at most: a cumulative sum's borders move by that).  The table's 32 doubles lie in each LDS bank once: no conflicts.  What is below 2^-1000 becomes
+// that (VF_NOTHING): beside a chunk's largest term it is gone, and weights are taken less twice as much, so that a masked token has none.
+constexpr double VF_NOTHING = 0x1p-1000;
+struct VfExp {
+  const double* table;
+  double C, E;                               // both times 32
+  __device__ __forceinline__ double operator()(float z) const {
+    constexpr double MAGIC = 6755399441055744.0, L = 0.69314718055994530942 / 32;   // 1.5 * 2^52: the sum's low bits are the whole number
+    const double y = fmax(fma((double)z, C, -E), -32000.0);
+    const double t = y + MAGIC, r = y - (t - MAGIC);
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+    double p = fma(r, L * L * L * L / 24, L * L * L / 6);
+    p = fma(r, p, L * L / 2);
+    p = fma(r, p, L);
+    p = fma(r, p, 1.0);
+    p *= table[n & 31];
+    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)((n & ~31u) << 15) << 32));   // k into the exponent
+  }
+};
+// probability of logit z in a row of sum `s`; what VF_NOTHING stands for is 0
+__device__ __forceinline__ double vf_prob(const double* table, double C, const VfSum& s, float z) {
+  const double e = VfExp{table, 32.0 * C, 32.0 * s.e}(z);
+  return e > 2.0 * VF_NOTHING ? e / s.s : 0.0;
+}
+__device__ __forceinline__ double vf_scaled(const VfSum& x, double e) { return x.e == e ? x.s : ldexp(x.s, (int)fmax(x.e - e, -4000.0)); }   // s 2^(x.e - e)
+__device__ __forceinline__ VfSum vf_add(const VfSum& x, const VfSum& y) {
+  const double e = fmax(x.e, y.e);
+  return VfSum{e, vf_scaled(x, e) + vf_scaled(y, e)};
+}
+__device__ __forceinline__ bool vf_good(const VfSum& x) { return x.e > -INFINITY && x.e < INFINITY && x.s > 0.0; }
+__device__ __forceinline__ double vf_ceil(float m, double C) { return m == -INFINITY ? 0.0 : ceil((double)m * C); }
 
+// (maximum, sum) of a share of one drafted position's row
 template <int DT>
 __global__ __launch_bounds__(VF_T) void verify_stats_kernel(VerifyArgs a) {
-  constexpr int VEC = Lg<DT>::VEC, U = 4;
+  constexpr int VEC = Lg<DT>::VEC, U = 32 / VEC;
   __shared__ MS red[VF_T / 64];
-  const int rows = a.draft ? 2 : 1;
-  uint32_t id = blockIdx.x;
-  const int split = (int)(id % (uint32_t)a.nsplit); id /= (uint32_t)a.nsplit;
-  const int which = (int)(id % (uint32_t)rows); id /= (uint32_t)rows;
-  const int b = (int)(id % (uint32_t)a.B), i = (int)(id / (uint32_t)a.B);
+  const int64_t row = blockIdx.x / (uint32_t)a.nstat, trows = (int64_t)a.B * a.K;
+  const int split = (int)(blockIdx.x % (uint32_t)a.nstat);
+  const int64_t of = row < trows ? row : row - trows;
+  const int b = (int)(of / a.K), i = (int)(of - (int64_t)b * a.K);
   if (i >= vf_drafts(a, b)) return;
-  const char* row = which ? a.draft + b * a.db + i * a.dp : a.target + b * a.tb + i * a.tp;
+  const char* z = row < trows ? a.target + b * a.tb + i * a.tp : a.draft + b * a.db + i * a.dp;
   const int nvec = (a.V + VEC - 1) / VEC;
-  const int v0 = (int)((int64_t)nvec * split / a.nsplit), v1 = (int)((int64_t)nvec * (split + 1) / a.nsplit);
+  const int v0 = (int)((int64_t)nvec * split / a.nstat), v1 = (int)((int64_t)nvec * (split + 1) / a.nstat);
   float m = -INFINITY, s = 0.0f;
   for (int v = v0; v < v1; v += VF_T * U) {
     Pack x[U];
+    if (v + VF_T * U <= v1 && (v + VF_T * U) * VEC <= a.V) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) { const int at = v + u * VF_T + (int)threadIdx.x; x[u] = at < v1 ? tk_load<DT>(row, at, a.V) : tk_neg<DT>(); }
+      for (int u = 0; u < U; ++u) x[u] = tk_load16(z + (size_t)(v + u * VF_T + (int)threadIdx.x) * 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) { const int at = v + u * VF_T + (int)threadIdx.x; x[u] = at < v1 ? tk_load<DT>(z, at, a.V) : tk_neg<DT>(); }
+    }
     float nm = m;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) nm = fmaxf(nm, tk_get<DT>(x[u], j));
-    const float base = tk_base(nm);
+    for (int u = 0; u < U; ++u) { nm = fmaxf(nm, tk_max<DT>(x[u])); tk_redecode(x[u]); }
+    const ExpSum es(tk_base(nm), a.c);
     float p = 0.0f;
+    if (!es.big) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) p += es.usual<DT>(x[u]);
+    } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) p += tk_exp2((tk_get<DT>(x[u], j) - base) * a.c);
-    s = s * tk_exp2((m - base) * a.c) + p;
+      for (int u = 0; u < U; ++u) p += es.large<DT>(x[u]);
+    }
+    s = s * tk_exp2((m - es.b) * a.c) + p * es.fix;
     m = nm;
   }
   const MS ms = block_lse<VF_T>(m, s, a.c, red);
   if (threadIdx.x == 0) a.stats[blockIdx.x] = ms;
 }
 
-// probability of `token` in a row whose statistics are split; NaN where the row is no distribution (nothing but -inf, a NaN, +inf)
-template <int DT> __device__ double vf_prob(const VerifyArgs& a, const MS* st, const char* row, int token, double* logp) {
-  float M = st[0].m;
-  for (int k = 1; k < a.nsplit; ++k) M = fmaxf(M, st[k].m);
-  double S = 0.0;
-  for (int k = 0; k < a.nsplit; ++k) S += st[k].s * (double)tk_exp2((st[k].m - tk_base(M)) * a.c);
-  if (!(M > -INFINITY && M < INFINITY)) return NAN;
-  const double x = ((double)tk_at<DT>(row, token) - (double)M) * a.inv_tau;
-  *logp = x - log(S);
-  return exp(x) / S;
-}
-
-template <int DT>
-__global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
-  constexpr int VEC = Lg<DT>::VEC, U = 16 / VEC;
-  __shared__ int sa;
-  __shared__ float sm[2][VF_T / 64];
-  __shared__ double ss[2][VF_T / 64];
+// How many drafts of sequence b are accepted; every thread of the block gets it.  srow: the rows' sums, target 0 .. n, draft 0 .. n - 1 behind them
+// (from fp32 statistics target 0 .. n - 1).  `write`: the block that writes what is known then.
+template <int DT, bool ALL> __device__ int vf_accept(const VerifyArgs& a, int b, int n, bool write, const double* table, VfSum* srow, int* sat) {
   const int tid = threadIdx.x;
-  const int b = (int)(blockIdx.x / (uint32_t)a.nchunk), ch = (int)(blockIdx.x % (uint32_t)a.nchunk);
-  const int n = vf_drafts(a, b);
-  if (tid == 0) sa = n;
+  const int64_t k0 = (int64_t)b * a.K, t0 = (int64_t)b * (a.K + 1);
+  int x = -1;
+  float u = 0.0f, zp = 0.0f, zq = 0.0f;
+  if (tid < n) {
+    x = a.tokens[k0 + tid];
+    u = a.u_accept[k0 + tid];
+    if ((uint32_t)x < (uint32_t)a.V) {
+      zp = tk_at<DT>(a.target + b * a.tb + tid * a.tp, x);
+      if (a.draft) zq = tk_at<DT>(a.draft + b * a.db + tid * a.dp, x);
+    }
+  }
+  if (tid == 0) *sat = n;
+  const int heads = ALL ? n + 1 : n, rows = heads + (a.draft ? n : 0);
+  for (int r = tid >> 4; r < rows; r += VF_T / 16) {   // 16 lanes a row
+    VfSum s = {-INFINITY, 0.0};
+    if constexpr (ALL) {
+      const VfSum* p = a.parts + (r < heads ? t0 + r : (int64_t)a.B * (a.K + 1) + k0 + r - heads) * a.nsplit;
+      for (int i = tid & 15; i < a.nsplit; i += 16) s = vf_add(s, p[i]);
+      for (int o = 8; o > 0; o >>= 1) s = vf_add(s, VfSum{__shfl_xor(s.e, o, 16), __shfl_xor(s.s, o, 16)});
+    } else {
+      const MS* p = a.stats + (r < heads ? k0 + r : (int64_t)a.B * a.K + k0 + r - heads) * a.nstat;
+      float m = -INFINITY;
+      for (int i = tid & 15; i < a.nstat; i += 16) m = fmaxf(m, p[i].m);
+      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
+      for (int i = tid & 15; i < a.nstat; i += 16) s.s += p[i].s * (double)tk_exp2((p[i].m - tk_base(m)) * a.c);
+      for (int o = 8; o > 0; o >>= 1) s.s += __shfl_xor(s.s, o, 16);
+      s.e = (double)m * a.C;
+    }
+    if ((tid & 15) == 0) srow[r] = s;
+  }
   __syncthreads();
   double logp = 0.0;
-  int x = -1;
   if (tid < n) {
-    x = a.tokens[(int64_t)b * a.K + tid];
     bool ok = false;
-    if ((uint32_t)x < (uint32_t)a.V) {
-      const int rows = a.draft ? 2 : 1;
-      const MS* st = a.stats + ((int64_t)(tid * a.B + b) * rows) * a.nsplit;
-      const double p = vf_prob<DT>(a, st, a.target + b * a.tb + tid * a.tp, x, &logp);
-      double q = 1.0, unused;
-      if (a.draft) q = vf_prob<DT>(a, st + a.nsplit, a.draft + b * a.db + tid * a.dp, x, &unused);
-      ok = (double)a.u_accept[(int64_t)b * a.K + tid] * q < p;   // (a NaN on either side: not accepted)
+    if ((uint32_t)x < (uint32_t)a.V && vf_good(srow[tid])) {
+      const VfSum ps = srow[tid];
+      const double p = vf_prob(table, a.C, ps, zp);
+      double q = 1.0;
+      if (a.draft) {
+        const VfSum qs = srow[heads + tid];
+        q = vf_good(qs) ? vf_prob(table, a.C, qs, zq) : NAN;
+      }
+      ok = (double)u * q < p;                // (a NaN: not accepted)
+      if (ok && write) logp = ((double)zp * a.C - ps.e) * 0.69314718055994530942 - log(ps.s);
     }
-    if (!ok) atomicMin(&sa, tid);
+    if (!ok) atomicMin(sat, tid);
   }
   __syncthreads();
-  const int at = sa;
-  if (ch == 0) {
-    if (tid < at) { a.out[(int64_t)b * (a.K + 1) + tid] = x; if (a.logprobs) a.logprobs[(int64_t)b * (a.K + 1) + tid] = (float)logp; }
-    else if (tid > at && tid <= a.K) { a.out[(int64_t)b * (a.K + 1) + tid] = -1; if (a.logprobs) a.logprobs[(int64_t)b * (a.K + 1) + tid] = 0.0f; }
+  const int at = *sat;
+  if (write) {
+    if (tid < at) { a.out[t0 + tid] = x; if (a.logprobs) a.logprobs[t0 + tid] = (float)logp; }
+    else if (tid > at && tid <= a.K) { a.out[t0 + tid] = -1; if (a.logprobs) a.logprobs[t0 + tid] = 0.0f; }
     if (tid == 0) a.accepted[b] = at;
   }
-  // the row that the next token is drawn from, and the draft's row where a token was rejected
-  const char* prow = a.target + b * a.tb + at * a.tp;
-  const char* qrow = a.draft && at < n ? a.draft + b * a.db + at * a.dp : nullptr;
-  const int skip = !a.draft && at < n ? a.tokens[(int64_t)b * a.K + at] : -1;   // a looked-up token that was rejected has no weight left
-  Pack px[U], qx[U];
+  return at;
+}
+
+// a chunk's vectors of a lane
+template <int DT> __device__ __forceinline__ void vf_chunk(Pack (&y)[VF_CHUNK / 64 / Lg<DT>::VEC], const char* row, int ch, int V) {
+  constexpr int U = VF_CHUNK / 64 / Lg<DT>::VEC;
+  const int lane = threadIdx.x & 63;
+  if ((ch + 1) * VF_CHUNK <= V) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int v = (ch * U + u) * VF_T + tid;
-    px[u] = tk_load<DT>(prow, v, a.V);
-    qx[u] = qrow ? tk_load<DT>(qrow, v, a.V) : tk_neg<DT>();
+    for (int u = 0; u < U; ++u) y[u] = tk_load16(row + (size_t)((ch * U + u) * 64 + lane) * 16);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) y[u] = tk_load<DT>(row, (ch * U + u) * 64 + lane, V);
   }
-  float mp = -INFINITY, mq = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { mp = fmaxf(mp, tk_get<DT>(px[u], j)); mq = fmaxf(mq, tk_get<DT>(qx[u], j)); }
-  mp = wave_max(mp); mq = wave_max(mq);
-  if ((tid & 63) == 0) { sm[0][tid >> 6] = mp; sm[1][tid >> 6] = mq; }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < VF_T / 64; ++i) { mp = fmaxf(mp, sm[0][i]); mq = fmaxf(mq, sm[1][i]); }
-  double sp = 0.0, sq = 0.0;
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const double e = exp(((double)tk_get<DT>(px[u], j) - (double)tk_base(mp)) * a.inv_tau);
-      if (((ch * U + u) * VF_T + tid) * VEC + j == skip) sq = e; else sp += e;
-      if (qrow) sq += exp(((double)tk_get<DT>(qx[u], j) - (double)tk_base(mq)) * a.inv_tau);
+}
+
+template <int DT, bool ALL>
+__global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
+  constexpr int VEC = Lg<DT>::VEC, U = VF_CHUNK / 64 / VEC;
+  __shared__ double table[32];
+  __shared__ VfSum part[VF_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x / (uint32_t)a.nsplit;
+  const int split = (int)(blockIdx.x % (uint32_t)a.nsplit);
+  const char* z;
+  if (tid < 32) table[tid] = exp2(tid / 32.0);
+  if constexpr (ALL) {
+    const int64_t trows = (int64_t)a.B * (a.K + 1);
+    if (row < trows) {
+      const int b = (int)(row / (a.K + 1)), i = (int)(row - (int64_t)b * (a.K + 1));
+      if (i == 0 && split == 0 && tid == 0) a.done[b] = 0;
+      if (i > vf_drafts(a, b)) return;
+      z = a.target + b * a.tb + i * a.tp;
+    } else {
+      const int b = (int)((row - trows) / a.K), i = (int)(row - trows - (int64_t)b * a.K);
+      if (i >= vf_drafts(a, b)) return;
+      z = a.draft + b * a.db + i * a.dp;
     }
-  sp = wave_sum(sp); sq = wave_sum(sq);
-  if ((tid & 63) == 0) { ss[0][tid >> 6] = sp; ss[1][tid >> 6] = sq; }
+  } else {
+    __shared__ VfSum srow[2 * TK_MAX_DRAFTS];
+    __shared__ int sat;
+    const bool of_draft = row >= a.B;
+    const int b = (int)(of_draft ? row - a.B : row), n = vf_drafts(a, b);
+    const int at = vf_accept<DT, false>(a, b, n, !of_draft && split == 0, table, srow, &sat);
+    if (!of_draft && split == 0 && tid == 0) a.done[b] = 0;
+    if (of_draft && at >= n) return;
+    z = of_draft ? a.draft + b * a.db + at * a.dp : a.target + b * a.tb + at * a.tp;
+  }
+  const int c0 = (int)((int64_t)a.nchunk * split / a.nsplit), c1 = (int)((int64_t)a.nchunk * (split + 1) / a.nsplit);
+  Pack y[U];
+  if (c0 + wave < c1) vf_chunk<DT>(y, z, c0 + wave, a.V);
+  __syncthreads();
+  VfSum all = {-INFINITY, 0.0};
+  for (int ch = c0 + wave; ch < c1; ch += VF_WAVES) {
+    Pack x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = y[u];
+    if (ch + VF_WAVES < c1) vf_chunk<DT>(y, z, ch + VF_WAVES, a.V);
+    float m = -INFINITY;
+    uint64_t nan = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m = fmaxf(m, tk_max<DT>(x[u]));
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) nan |= __ballot(__builtin_isunordered(tk_get<DT>(x[u], j), tk_get<DT>(x[u], j + 1)));
+    }
+    m = wave_max(m);
+    const double E = vf_ceil(m, a.C);
+    const VfExp ex = {table, 32.0 * a.C, 32.0 * E};
+    double s = 0.0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if ((ch * U + u) * 64 * VEC >= a.V) break;   // (the same for every lane)
+      tk_redecode(x[u]);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s += ex(tk_get<DT>(x[u], j));
+    }
+    s = wave_sum(s);
+    if (m == -INFINITY) s = 0.0;
+    if (nan) s = NAN;
+    const VfSum mine = {m == -INFINITY ? -INFINITY : E, s};
+    if (lane == 0) a.sums[row * a.nchunk + ch] = mine;
+    all = vf_add(all, mine);
+  }
+  if (lane == 0) part[wave] = all;
   __syncthreads();
   if (tid == 0) {
-    sp = sq = 0.0;
-    for (int i = 0; i < VF_T / 64; ++i) { sp += ss[0][i]; sq += ss[1][i]; }
-    a.sums[blockIdx.x] = VfSum{sp, sq, mp, mq};
+    for (int w = 1; w < VF_WAVES; ++w) all = vf_add(all, part[w]);
+    a.parts[row * a.nsplit + split] = all;
   }
 }
 
-// a sequence's row as a whole: maximum, sum, and whether it is a distribution
-struct VfRow { double m, s; bool good; };
-__device__ __forceinline__ VfRow vf_row(const VerifyArgs& a, int b, bool q) {
-  const VfSum* s = a.sums + (int64_t)b * a.nchunk;
-  float M = -INFINITY;
-  for (int i = 0; i < a.nchunk; ++i) M = fmaxf(M, q ? s[i].mq : s[i].mp);
-  double S = 0.0;
-  for (int i = 0; i < a.nchunk; ++i) S += (q ? s[i].q : (a.draft ? s[i].p : s[i].p + s[i].q)) * exp(((double)(q ? s[i].mq : s[i].mp) - (double)tk_base(M)) * a.inv_tau);
-  return VfRow{(double)M, S, M > -INFINITY && M < INFINITY && S > 0.0};
-}
-// the weight of a token: p, max(p - q, 0), or p without the rejected token of a looked-up draft
-struct VfWeight {
-  double inv_tau, pm, pn, qm, qn;            // pn, qn: 1 / sum
-  int skip;                                  // a token of no weight, or -1
-  bool q;
-  __device__ double operator()(float zp, float zq, int e) const {
-    const double p = exp(((double)zp - pm) * inv_tau) * pn;
-    if (q) { const double d = p - exp(((double)zq - qm) * inv_tau) * qn; return d > 0.0 ? d : 0.0; }
-    return e == skip ? 0.0 : p;
-  }
-};
-
-template <int DT>
-__global__ __launch_bounds__(VF_T) void verify_rest_kernel(VerifyArgs a) {
-  constexpr int VEC = Lg<DT>::VEC, U = 16 / VEC;
-  __shared__ double ss[VF_T / 64];
-  __shared__ VfRow srow[2];
-  const int tid = threadIdx.x;
-  const int b = (int)(blockIdx.x / (uint32_t)a.nchunk), ch = (int)(blockIdx.x % (uint32_t)a.nchunk);
-  const int at = a.accepted[b];
-  if (at >= vf_drafts(a, b)) return;
-  if (tid < 2) srow[tid] = vf_row(a, b, tid == 1);
+// inclusive sum over the block's threads, and the whole; `ss` holds one number a wave
+__device__ double vf_scan(double v, double* ss, double* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(v, d, 64); if (lane >= d) v += o; }
   __syncthreads();
-  if (!srow[0].good || !srow[1].good) return;
-  const VfWeight w = {a.inv_tau, srow[0].m, 1.0 / srow[0].s, srow[1].m, 1.0 / srow[1].s, -1, true};
-  const char* prow = a.target + b * a.tb + at * a.tp;
-  const char* qrow = a.draft + b * a.db + at * a.dp;
-  double s = 0.0;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int v = (ch * U + u) * VF_T + tid;
-    const Pack px = tk_load<DT>(prow, v, a.V), qx = tk_load<DT>(qrow, v, a.V);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) s += w(tk_get<DT>(px, j), tk_get<DT>(qx, j), 0);
-  }
-  s = wave_sum(s);
-  if ((tid & 63) == 0) ss[tid >> 6] = s;
+  if (lane == 63) ss[wave] = v;
   __syncthreads();
-  if (tid == 0) { s = 0.0; for (int i = 0; i < VF_T / 64; ++i) s += ss[i]; a.rest[blockIdx.x] = s; }
+  double t = 0.0;
+#pragma unroll
+  for (int w = 0; w < VF_WAVES; ++w) { if (w == wave) v += t; t += ss[w]; }
+  *total = t;
+  return v;
 }
 
-template <int DT>
+template <int DT, bool ALL>
 __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
-  constexpr int PER = VF_CHUNK / VF_T;       // neighbouring tokens a thread
-  __shared__ VfRow srow[2];
-  __shared__ VfWeight sweight;
-  __shared__ double sbelow, sgoal, ss[VF_T / 64];
-  __shared__ int schunk, stoken, slast;
-  const int tid = threadIdx.x, b = blockIdx.x;
-  const int n = vf_drafts(a, b), at = a.accepted[b];
+  constexpr int VEC = Lg<DT>::VEC, U = VF_CHUNK / 64 / VEC;
+  __shared__ double table[32];
+  __shared__ double ss[VF_WAVES];
+  __shared__ VfSum srow[ALL ? 2 * TK_MAX_DRAFTS + 1 : 2];
+  __shared__ int sat, sfirst, slast, slastblock;
+  __shared__ double sbelow;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = (int)(blockIdx.x / (uint32_t)a.npick), part = (int)(blockIdx.x % (uint32_t)a.npick);
+  const int n = vf_drafts(a, b);
+  if (tid < 32) table[tid] = exp2(tid / 32.0);
+  int at, prow_at, qrow_at;                  // drafts accepted; where srow holds the row that the token is drawn from, and the draft's
+  int64_t prow_id;                           // which row of `sums` it is
+  if constexpr (ALL) {
+    at = vf_accept<DT, true>(a, b, n, part == 0, table, srow, &sat);
+    prow_at = at; qrow_at = n + 1 + at;
+    prow_id = (int64_t)b * (a.K + 1) + at;
+  } else {
+    at = a.accepted[b];
+    prow_at = 0; qrow_at = 1;
+    prow_id = b;
+    if (tid < 32 && (tid < 16 || (a.draft && at < n))) {
+      const VfSum* p = a.parts + (int64_t)(tid < 16 ? b : a.B + b) * a.nsplit;
+      VfSum s = {-INFINITY, 0.0};
+      for (int i = tid & 15; i < a.nsplit; i += 16) s = vf_add(s, p[i]);
+      for (int o = 8; o > 0; o >>= 1) s = vf_add(s, VfSum{__shfl_xor(s.e, o, 16), __shfl_xor(s.s, o, 16)});
+      if ((tid & 15) == 0) srow[tid >> 4] = s;
+    }
+    __syncthreads();
+  }
   const int64_t o = (int64_t)b * (a.K + 1) + at;
-  const char* prow = a.target + b * a.tb + at * a.tp;
-  const char* qrow = a.draft && at < n ? a.draft + b * a.db + at * a.dp : nullptr;
-  const VfSum* sums = a.sums + (int64_t)b * a.nchunk;
-  if (tid == 0 || (tid == 1 && qrow)) srow[tid] = vf_row(a, b, tid == 1);
-  if (tid == 0) { stoken = a.V; slast = -1; }
-  __syncthreads();
-  if (!srow[0].good) {                       // no distribution to draw from
-    if (tid == 0) { a.out[o] = -1; if (a.logprobs) a.logprobs[o] = 0.0f; }
+  const VfSum ps = srow[prow_at];
+  if (!vf_good(ps)) {                        // no distribution to draw from
+    if (part == 0 && tid == 0) { a.out[o] = -1; if (a.logprobs) a.logprobs[o] = 0.0f; }
     return;
   }
-  if (tid == 0) {
-    VfWeight w = {a.inv_tau, srow[0].m, 1.0 / srow[0].s, 0.0, 0.0, -1, false};
-    const int x = at < n ? a.tokens[(int64_t)b * a.K + at] : -1;
-    if (qrow && srow[1].good) {
-      w.q = true; w.qm = srow[1].m; w.qn = 1.0 / srow[1].s;
-      double total = 0.0;
-      for (int i = 0; i < a.nchunk; ++i) total += a.rest[(int64_t)b * a.nchunk + i];
-      if (!(total > 0.0)) w.q = false;       // p nowhere above q
-    } else if (!a.draft && (uint32_t)x < (uint32_t)a.V) w.skip = x;
-    double total = 0.0;
-    const auto chunk = [&](int i) {
-      if (w.q) return a.rest[(int64_t)b * a.nchunk + i];
-      return (!a.draft && w.skip < 0 ? sums[i].p + sums[i].q : sums[i].p) * exp(((double)sums[i].mp - w.pm) * a.inv_tau) * w.pn;
-    };
-    for (int i = 0; i < a.nchunk; ++i) total += chunk(i);
-    if (!(total > 0.0)) { w.skip = -1; total = 0.0; for (int i = 0; i < a.nchunk; ++i) total += chunk(i); }
-    const float u = a.u_sample[b];
-    const double goal = (u > 0.0f ? (double)u : 0.0) * total;
-    double below = 0.0, start = 0.0;
-    int hit = -1;
-    for (int i = 0; i < a.nchunk; ++i) {     // the first chunk that ends above the goal; the last one with weight where rounding (or u >= 1) leaves none
-      const double s = chunk(i);
-      if (s > 0.0) {
-        hit = i; start = below;
-        if (below + s > goal) break;
+  const char* prow = a.target + b * a.tb + at * a.tp;
+  const char* qrow = a.draft && at < n && vf_good(srow[qrow_at]) ? a.draft + b * a.db + at * a.dp : nullptr;
+  const VfSum qs = qrow ? srow[qrow_at] : VfSum{0.0, 1.0};
+  const VfExp ep = {table, 32.0 * a.C, 32.0 * ps.e}, eq = {table, 32.0 * a.C, 32.0 * qs.e};
+  const double np = 1.0 / ps.s, nq = 1.0 / qs.s, none = 2.0 * VF_NOTHING * np;
+  bool rest = qrow != nullptr;
+  if (rest) {
+    for (int ch = part * VF_WAVES + wave; ch < a.nchunk; ch += a.npick * VF_WAVES) {
+      Pack px[U], qx[U];
+      vf_chunk<DT>(px, prow, ch, a.V);
+      vf_chunk<DT>(qx, qrow, ch, a.V);
+      double s = 0.0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if ((ch * U + u) * 64 * VEC >= a.V) break;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += fmax(fma(ep(tk_get<DT>(px[u], j)), np, fma(eq(tk_get<DT>(qx[u], j)), -nq, -none)), 0.0);
       }
-      below += s;
+      s = wave_sum(s);
+      if (lane == 0) __hip_atomic_store(&a.rest[(int64_t)b * a.nchunk + ch], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    schunk = hit; sbelow = start; sgoal = goal; sweight = w;
-  }
-  __syncthreads();
-  const VfWeight w = sweight;
-  const int e0 = schunk * VF_CHUNK + tid * PER;
-  double t[PER], s = 0.0;
+    if (a.npick > 1) {                       // the last block to come by sees what all have written: the sums are written through and read past the caches
+                                             // (agent scope), each wave waits for its own, then the block counts; a whole-cache write-back per block cost 100 us
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (tid == 0) slastblock = __hip_atomic_fetch_add(&a.done[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)a.npick - 1;
+      __syncthreads();
+      if (!slastblock) return;
+    } else __syncthreads();
+  } else if (part != 0) return;
+
+  // the chunk that the goal falls into; a thread looks at neighbouring chunks
+  const int rejected = !a.draft && at < n ? a.tokens[(int64_t)b * a.K + at] : -1;
+  int skip = (uint32_t)rejected < (uint32_t)a.V ? rejected : -1;   // a looked-up token that was rejected has no weight left
+  const auto weight = [&](int e) {
+    if (e >= a.V || e == skip) return 0.0;
+    return fmax(fma(ep(tk_at<DT>(prow, e)), np, rest ? fma(eq(tk_at<DT>(qrow, e)), -nq, -none) : -none), 0.0);
+  };
+  const VfSum* sums = a.sums + prow_id * a.nchunk;
+  const int per = (a.nchunk + VF_T - 1) / VF_T;
+  const float u = a.u_sample[b];
+  double total, goal, before;
+  for (;;) {
+    double without = 0.0;                    // the skipped token's chunk, summed again without it
+    if (skip >= 0) {
+      double w = 0.0;
+      for (int j = 0; j < VF_CHUNK / VF_T; ++j) w += weight(skip / VF_CHUNK * VF_CHUNK + tid * (VF_CHUNK / VF_T) + j);
+      (void)vf_scan(w, ss, &without);
+    }
+    const auto chunk = [&](int i) {
+      if (i >= a.nchunk) return 0.0;
+      if (rest) return (double)__hip_atomic_load(&a.rest[(int64_t)b * a.nchunk + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return skip >= 0 && i == skip / VF_CHUNK ? without : vf_scaled(sums[i], ps.e) * np;
+    };
+    double mine = 0.0;
+    for (int j = 0; j < per; ++j) mine += chunk(tid * per + j);
+    before = vf_scan(mine, ss, &total) - mine;
+    if (!(total > 0.0) && (rest || skip >= 0)) { rest = false; skip = -1; continue; }   // nothing left of p: p itself
+    if (tid == 0) { sfirst = a.nchunk; slast = -1; }
+    __syncthreads();
+    goal = (u > 0.0f ? (double)u : 0.0) * total;
+    double c = before;
+    int first = a.nchunk, last = -1;
+    for (int j = 0; j < per; ++j) {
+      const double w = chunk(tid * per + j);
+      c += w;
+      if (w > 0.0) { last = tid * per + j; if (c > goal && first == a.nchunk) first = last; }
+    }
+    if (first < a.nchunk) atomicMin(&sfirst, first);
+    if (last >= 0) atomicMax(&slast, last);
+    __syncthreads();
+    const int hit = sfirst < a.nchunk ? sfirst : slast;   // (rounding, or u >= 1, may leave no sum above the goal: the last weight there is)
+    if (hit / per == tid) { c = before; for (int j = tid * per; j < hit; ++j) c += chunk(j); sbelow = c; }
+    __syncthreads();
+    // the token inside the chunk
+    constexpr int PER = VF_CHUNK / VF_T;
+    const int e0 = hit * VF_CHUNK + tid * PER;
+    double t[PER], s = 0.0, sum;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int e = e0 + j;
-    t[j] = e < a.V ? w(tk_at<DT>(prow, e), w.q ? tk_at<DT>(qrow, e) : 0.0f, e) : 0.0;
-    s += t[j];
-  }
-  // exclusive sum over the threads before
-  double inc = s;
-  for (int d = 1; d < 64; d <<= 1) { const double v = __shfl_up(inc, d, 64); if ((tid & 63) >= d) inc += v; }
-  if ((tid & 63) == 63) ss[tid >> 6] = inc;
-  __syncthreads();
-  double c = sbelow + (inc - s);
-  for (int i = 0; i < (tid >> 6); ++i) c += ss[i];
-  int first = a.V, last = -1;
+    for (int j = 0; j < PER; ++j) { t[j] = weight(e0 + j); s += t[j]; }
+    c = sbelow + (vf_scan(s, ss, &sum) - s);
+    if (tid == 0) { sfirst = a.V; slast = -1; }
+    __syncthreads();
+    first = a.V; last = -1;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    c += t[j];
-    if (t[j] > 0.0) { last = e0 + j; if (c > sgoal && first == a.V) first = e0 + j; }
+    for (int j = 0; j < PER; ++j) {
+      c += t[j];
+      if (t[j] > 0.0) { last = e0 + j; if (c > goal && first == a.V) first = last; }
+    }
+    if (first < a.V) atomicMin(&sfirst, first);
+    if (last >= 0) atomicMax(&slast, last);
+    __syncthreads();
+    break;
   }
-  if (first < a.V) atomicMin(&stoken, first);
-  if (last >= 0) atomicMax(&slast, last);
-  __syncthreads();
   if (tid == 0) {
-    const int token = stoken < a.V ? stoken : slast;
+    const int token = sfirst < a.V ? sfirst : slast;
     a.out[o] = token;
-    if (a.logprobs) a.logprobs[o] = token < 0 ? 0.0f : (float)(((double)tk_at<DT>(prow, token) - srow[0].m) * a.inv_tau - log(srow[0].s));
+    if (a.logprobs) a.logprobs[o] = (float)(((double)tk_at<DT>(prow, token) * a.C - ps.e) * 0.69314718055994530942 - log(ps.s));
   }
 }
 
 // tau = 0: p is one-hot at the row's largest logit (the lowest index of equal ones), a draft is accepted where it is that token
 struct VfBest { float m; int32_t idx, bad, pad; };   // bad: a NaN or +inf among the logits
-static_assert(sizeof(VfBest) == sizeof(MS), "both live in the same part of the workspace");
 __device__ __forceinline__ void vf_better(float& m, int& idx, float om, int oi) { if (om > m || (om == m && oi < idx)) { m = om; idx = oi; } }
 
 template <int DT>
@@ -911,7 +1154,7 @@ __global__ __launch_bounds__(VF_T) void verify_best_kernel(VerifyArgs a) {
   __syncthreads();
   if (tid == 0) {
     for (int k = 1; k < VF_T / 64; ++k) { vf_better(m, idx, red[k].m, red[k].idx); bad |= red[k].bad; }
-    reinterpret_cast<VfBest*>(a.stats)[blockIdx.x] = VfBest{m, idx, bad, 0};
+    reinterpret_cast<VfBest*>(a.sums)[blockIdx.x] = VfBest{m, idx, bad, 0};
   }
 }
 __global__ __launch_bounds__(VF_T) void verify_greedy_kernel(VerifyArgs a) {
@@ -921,7 +1164,7 @@ __global__ __launch_bounds__(VF_T) void verify_greedy_kernel(VerifyArgs a) {
   __syncthreads();
   int best = -1;
   if (tid <= n) {
-    const VfBest* st = reinterpret_cast<const VfBest*>(a.stats) + ((int64_t)tid * a.B + b) * a.nsplit;
+    const VfBest* st = reinterpret_cast<const VfBest*>(a.sums) + ((int64_t)tid * a.B + b) * a.nsplit;
     float m = -INFINITY;
     int idx = a.V, bad = 0;
     for (int k = 0; k < a.nsplit; ++k) { vf_better(m, idx, st[k].m, st[k].idx); bad |= st[k].bad; }
@@ -936,32 +1179,43 @@ __global__ __launch_bounds__(VF_T) void verify_greedy_kernel(VerifyArgs a) {
   if (tid == 0) a.accepted[b] = sa;
 }
 
-struct VerifyPlan { int nsplit, nchunk; size_t o_sums, o_rest, ws; };
-VerifyPlan verify_plan(int B, int K, int V, int es, bool draft, bool greedy) {
-  VerifyPlan p;
-  const int nvec = (int)(((int64_t)V * es + 15) / 16);
-  const int64_t rows = greedy ? (int64_t)B * (K + 1) : (int64_t)B * K * (draft ? 2 : 1);
-  // about 1024 blocks in all, a share of at least 1024 vectors each
-  int64_t n = rows > 0 ? (1024 + rows - 1) / rows : 1;
-  const int most = (nvec + 1023) / 1024;
-  p.nsplit = (int)(n < most ? n : most);
+struct VerifyPlan { bool all; int nchunk, nstat, nsplit, npick; size_t o_parts, o_rest, o_stats, o_done, ws; };
+VerifyPlan verify_plan(int B, int K, int V, bool draft, bool greedy) {
+  VerifyPlan p = {};
   p.nchunk = (V + VF_CHUNK - 1) / VF_CHUNK;
-  p.o_sums = (size_t)rows * p.nsplit * sizeof(MS);
-  p.o_rest = p.o_sums + (greedy ? 0 : (size_t)B * p.nchunk * sizeof(VfSum));
-  p.ws = p.o_rest + (greedy ? 0 : (size_t)B * p.nchunk * sizeof(double));
+  const int64_t all = (int64_t)B * (K + 1) + (draft && !greedy ? (int64_t)B * K : 0);
+  // fp64 sums of every row up to 2^24 logits (about 12 us of fp64 beside a launch saved of 5); beyond, of the rows that tokens are drawn from
+  p.all = greedy || K == 0 || all * V <= (1 << 24);
+  const int64_t rows = p.all ? all : (int64_t)B * (draft ? 2 : 1);
+  const int most = (p.nchunk + VF_WAVES - 1) / VF_WAVES;   // a chunk a wave
+  // blocks: about 16384 of the fp64 sums, 1024 in the last kernel, 8192 of the fp32 statistics
+  const auto share = [](int64_t blocks, int64_t of, int most) { const int64_t n = (blocks + of - 1) / of; return (int)(n < most ? n : most); };
+  p.nsplit = share(16384, rows, most);
+  p.npick = draft && K > 0 ? share(1024, B, most) : 1;
+  p.nstat = p.all ? 0 : share(8192, all, (V + 8191) / 8192);
+  if (greedy) { p.ws = (size_t)rows * p.nsplit * sizeof(VfBest); return p; }
+  p.o_parts = (size_t)rows * p.nchunk * sizeof(VfSum);
+  p.o_rest = p.o_parts + (size_t)rows * p.nsplit * sizeof(VfSum);
+  p.o_stats = p.o_rest + (size_t)B * p.nchunk * sizeof(double);
+  p.o_done = p.o_stats + (size_t)B * K * (draft ? 2 : 1) * p.nstat * sizeof(MS);
+  p.ws = p.o_done + (size_t)B * sizeof(uint32_t);
   return p;
 }
-template <int DT> void verify_dispatch(const VerifyArgs& a, bool greedy, hipStream_t st) {
+template <int DT> void verify_dispatch(const VerifyArgs& a, const VerifyPlan& p, bool greedy, hipStream_t st) {
   if (greedy) {
     hipLaunchKernelGGL(verify_best_kernel<DT>, dim3((uint32_t)((int64_t)a.B * (a.K + 1) * a.nsplit)), dim3(VF_T), 0, st, a);
     hipLaunchKernelGGL(verify_greedy_kernel, dim3(a.B), dim3(VF_T), 0, st, a);
     return;
   }
-  const uint32_t rows = (uint32_t)((int64_t)a.B * a.K * (a.draft ? 2 : 1));
-  if (rows) hipLaunchKernelGGL(verify_stats_kernel<DT>, dim3(rows * (uint32_t)a.nsplit), dim3(VF_T), 0, st, a);
-  hipLaunchKernelGGL(verify_sums_kernel<DT>, dim3((uint32_t)a.B * a.nchunk), dim3(VF_T), 0, st, a);
-  if (a.draft && a.K > 0) hipLaunchKernelGGL(verify_rest_kernel<DT>, dim3((uint32_t)a.B * a.nchunk), dim3(VF_T), 0, st, a);
-  hipLaunchKernelGGL(verify_pick_kernel<DT>, dim3(a.B), dim3(VF_T), 0, st, a);
+  const int64_t rows = (int64_t)a.B * (p.all ? a.K + 1 : 1) + (a.draft ? (int64_t)a.B * (p.all ? a.K : 1) : 0);
+  if (p.all) {
+    hipLaunchKernelGGL((verify_sums_kernel<DT, true>), dim3((uint32_t)(rows * a.nsplit)), dim3(VF_T), 0, st, a);
+    hipLaunchKernelGGL((verify_pick_kernel<DT, true>), dim3((uint32_t)a.B * a.npick), dim3(VF_T), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(verify_stats_kernel<DT>, dim3((uint32_t)((int64_t)a.B * a.K * (a.draft ? 2 : 1) * a.nstat)), dim3(VF_T), 0, st, a);
+    hipLaunchKernelGGL((verify_sums_kernel<DT, false>), dim3((uint32_t)(rows * a.nsplit)), dim3(VF_T), 0, st, a);
+    hipLaunchKernelGGL((verify_pick_kernel<DT, false>), dim3((uint32_t)a.B * a.npick), dim3(VF_T), 0, st, a);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ entry points: checks, plan, launches
@@ -1008,7 +1262,7 @@ constexpr double TK_LOG2E = 1.4426950408889634074;
 extern "C" int64_t cbm_top_logits_workspace(int32_t dtype, int32_t rows, int32_t vocab, int32_t k) {
   if (tk_rows("cbm_top_logits_workspace", dtype, rows, vocab)) return -1;
   if (k < 1 || k > TK_MAX_TOP) TK_REFUSE("cbm_top_logits_workspace: k %d outside [1, %d]", k, TK_MAX_TOP);
-  return rows ? (int64_t)top_plan(rows, vocab, k, tk_es(dtype)).ws : 0;
+  return rows ? (int64_t)top_plan(rows, vocab, k).ws : 0;
 }
 extern "C" int cbm_top_logits(cbm_ctx* c, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, int32_t k,
                               float temperature, int32_t* idx, float* values, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -1020,7 +1274,7 @@ extern "C" int cbm_top_logits(cbm_ctx* c, const void* logits, int32_t dtype, int
   if (rows == 0) { if (!c) TK_REFUSE("%s: null context", fn); return 0; }
   const int es = tk_es(dtype);
   if (tk_pointer(fn, "logits", logits, es) || tk_pointer(fn, "idx", idx, 4) || tk_pointer(fn, "values", values, 4) || tk_pointer(fn, "lse", lse, 4)) return -1;
-  const TopPlan p = top_plan(rows, vocab, k, es);
+  const TopPlan p = top_plan(rows, vocab, k);
   if (tk_workspace(fn, workspace, workspace_bytes, p.ws)) return -1;
   if (!c) TK_REFUSE("%s: null context", fn);
   DeviceScope dev(c);
@@ -1029,12 +1283,12 @@ extern "C" int cbm_top_logits(cbm_ctx* c, const void* logits, int32_t dtype, int
   a.logits = (const char*)logits; a.ld = row_stride * es;
   a.idx = idx; a.val = values; a.lse = lse;
   a.ws_keys = (uint64_t*)workspace; a.ws_ms = (MS*)((char*)workspace + (size_t)rows * p.nsplit * k * 8);
-  a.V = vocab; a.K = k; a.nsplit = p.nsplit; a.cap = p.cap;
+  a.V = vocab; a.K = k; a.rows = rows; a.nsplit = p.nsplit; a.cap = p.cap;
   a.inv_tau = 1.0 / (double)temperature; a.c = (float)(TK_LOG2E * a.inv_tau);
   hipStream_t st = tk_stream(c, stream);
-  if (dtype == CBM_F32) top_dispatch<CBM_F32>(a, rows, p, st);
-  else if (dtype == CBM_BF16) top_dispatch<CBM_BF16>(a, rows, p, st);
-  else top_dispatch<CBM_F16>(a, rows, p, st);
+  if (dtype == CBM_F32) top_dispatch<CBM_F32>(a, p, st);
+  else if (dtype == CBM_BF16) top_dispatch<CBM_BF16>(a, p, st);
+  else top_dispatch<CBM_F16>(a, p, st);
   return tk_done(fn);
 }
 
@@ -1082,7 +1336,7 @@ static int verify_check(const char* fn, int dtype, int B, int K, int V, float te
 }
 extern "C" int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, float temperature) {
   if (verify_check("cbm_verify_drafts_workspace", dtype, batch, drafts, vocab, temperature)) return -1;
-  return batch ? (int64_t)verify_plan(batch, drafts, vocab, tk_es(dtype), with_draft_logits != 0, temperature == 0.0f).ws : 0;
+  return batch ? (int64_t)verify_plan(batch, drafts, vocab, with_draft_logits != 0, temperature == 0.0f).ws : 0;
 }
 extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab,
                                  int64_t target_batch_stride, int64_t target_pos_stride, const void* draft_logits, int64_t draft_batch_stride,
@@ -1102,7 +1356,7 @@ extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t 
   if (!greedy && tk_pointer(fn, "u_sample", u_sample, 4)) return -1;
   if (draft_logits && tk_pointer(fn, "draft_logits", draft_logits, es)) return -1;
   if (drafts == 0 || greedy) draft_logits = nullptr;   // (not looked at)
-  const VerifyPlan p = verify_plan(batch, drafts, vocab, es, draft_logits != nullptr, greedy);
+  const VerifyPlan p = verify_plan(batch, drafts, vocab, draft_logits != nullptr, greedy);
   if (tk_workspace(fn, workspace, workspace_bytes, p.ws)) return -1;
   if (!c) TK_REFUSE("%s: null context", fn);
   DeviceScope dev(c);
@@ -1112,12 +1366,13 @@ extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t 
   a.draft = (const char*)draft_logits; a.db = draft_batch_stride * es; a.dp = draft_pos_stride * es;
   a.tokens = draft_tokens; a.n_draft = n_draft; a.u_accept = u_accept; a.u_sample = u_sample;
   a.out = tokens; a.accepted = accepted; a.logprobs = logprobs;
-  a.stats = (MS*)workspace; a.sums = (VfSum*)((char*)workspace + p.o_sums); a.rest = (double*)((char*)workspace + p.o_rest);
-  a.B = batch; a.K = drafts; a.V = vocab; a.nsplit = p.nsplit; a.nchunk = p.nchunk;
-  a.inv_tau = greedy ? 1.0 : 1.0 / (double)temperature; a.c = (float)(TK_LOG2E * a.inv_tau);
+  char* ws = (char*)workspace;
+  a.sums = (VfSum*)ws; a.parts = (VfSum*)(ws + p.o_parts); a.rest = (double*)(ws + p.o_rest); a.stats = (MS*)(ws + p.o_stats); a.done = (uint32_t*)(ws + p.o_done);
+  a.B = batch; a.K = drafts; a.V = vocab; a.nsplit = p.nsplit; a.nchunk = p.nchunk; a.nstat = p.nstat; a.npick = p.npick;
+  a.C = greedy ? 0.0 : TK_LOG2E / (double)temperature; a.c = (float)a.C;
   hipStream_t st = tk_stream(c, stream);
-  if (dtype == CBM_F32) verify_dispatch<CBM_F32>(a, greedy, st);
-  else if (dtype == CBM_BF16) verify_dispatch<CBM_BF16>(a, greedy, st);
-  else verify_dispatch<CBM_F16>(a, greedy, st);
+  if (dtype == CBM_F32) verify_dispatch<CBM_F32>(a, p, greedy, st);
+  else if (dtype == CBM_BF16) verify_dispatch<CBM_BF16>(a, p, greedy, st);
+  else verify_dispatch<CBM_F16>(a, p, greedy, st);
   return tk_done(fn);
 }

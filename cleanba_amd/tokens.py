@@ -18,26 +18,34 @@ import torch
 from . import lib as L
 
 _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_empty, _i32, _f32 = torch.empty, torch.int32, torch.float32
+try:   # the handle alone: a Stream object costs 2 us, as much as the launch
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:   # a build of torch without it
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 def _logits(ctx, t, name, dims=None):
+    """CBM_ type of a tensor of logits."""
     if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPE:
         raise ValueError(f"{name}: a float32, bfloat16 or float16 tensor is expected")
-    if t.dim() < 1 or (dims is not None and t.dim() != dims):
-        raise ValueError(f"{name}: {dims or 'one or more'} dimensions are expected, got {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
+    shape = t.shape
+    if not shape or (dims is not None and len(shape) != dims):
+        raise ValueError(f"{name}: {dims or 'one or more'} dimensions are expected, got {tuple(shape)}")
+    if t.stride(-1) != 1 and shape[-1] > 1 and t.numel():
         raise ValueError(f"{name}: the vocabulary (the last axis) has to be dense, its stride is {t.stride(-1)}")
     _placed(ctx, t, name)
     return _DTYPE[t.dtype]
 
 
 def _placed(ctx, t, name):
-    if t.device.type != "cuda" or t.device.index != ctx.cfg.device:
+    if not t.is_cuda or t.get_device() != ctx.cfg.device:
         raise ValueError(f"{name}: on {t.device}, the context's device is cuda:{ctx.cfg.device}")
 
 
 def _operand(ctx, t, name, dtype, shape):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: a {str(dtype)[6:]} tensor of shape {tuple(shape)} is expected, got "
                          f"{(str(t.dtype)[6:], tuple(t.shape)) if isinstance(t, torch.Tensor) else type(t).__name__}")
     _placed(ctx, t, name)
@@ -46,9 +54,10 @@ def _operand(ctx, t, name, dtype, shape):
 
 def _rows(t, name):
     """(rows, elements from row to row) of [..., vocab]; the leading axes have to fold into one."""
-    if t.dim() == 1:
+    dims = t.dim()
+    if dims == 1:
         return 1, t.shape[0]
-    if t.dim() > 2:
+    if dims > 2:
         try:
             t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(t.shape[:-1].numel(), t.shape[-1])
         except RuntimeError:
@@ -59,7 +68,7 @@ def _rows(t, name):
 def _workspace(nbytes, device):
     if nbytes < 0:
         raise L.CbmError(L.load().cbm_last_error().decode())
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return _empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _ptr(t):
@@ -71,13 +80,14 @@ def top_logits(ctx, logits, k, temperature=1.0):
     lse float32 [...] = log sum exp(logits / temperature)).  Slots beyond the logits above -inf hold -1 and -inf (cbm_top_logits)."""
     dtype = _logits(ctx, logits, "logits")
     rows, stride = _rows(logits, "logits")
-    vocab, lead, dev, k = logits.shape[-1], logits.shape[:-1], logits.device, int(k)
+    shape, dev, k = logits.shape, logits.device, int(k)
+    vocab, lead = shape[-1], shape[:-1]
     ws = _workspace(ctx.lib.cbm_top_logits_workspace(dtype, rows, vocab, k), dev)
-    idx = torch.empty(lead + (k,), dtype=torch.int32, device=dev)
-    values = torch.empty(lead + (k,), dtype=torch.float32, device=dev)
-    lse = torch.empty(lead, dtype=torch.float32, device=dev)
+    idx = _empty(lead + (k,), dtype=_i32, device=dev)
+    values = _empty(lead + (k,), dtype=_f32, device=dev)
+    lse = _empty(lead, dtype=_f32, device=dev)
     L._chk(ctx.lib.cbm_top_logits(ctx.h, logits.data_ptr(), dtype, rows, vocab, stride, k, temperature, idx.data_ptr(), values.data_ptr(), lse.data_ptr(),
-                                  _ptr(ws), 0 if ws is None else ws.numel(), torch.cuda.current_stream(dev).cuda_stream))
+                                  _ptr(ws), 0 if ws is None else ws.numel(), _raw_stream(ctx.cfg.device)))
     return idx, values, lse
 
 
@@ -89,7 +99,8 @@ def distill_loss_grad(ctx, logits, teacher_idx, teacher_logits, teacher_lse=None
     (cbm_distill_loss_grad)"""
     dtype = _logits(ctx, logits, "logits")
     rows, stride = _rows(logits, "logits")
-    vocab, lead, dev = logits.shape[-1], logits.shape[:-1], logits.device
+    shape, dev = logits.shape, logits.device
+    vocab, lead = shape[-1], shape[:-1]
     if not isinstance(teacher_idx, torch.Tensor) or teacher_idx.dim() != logits.dim():
         raise ValueError(f"teacher_idx: an int32 tensor of shape {tuple(lead) + ('k',)} is expected")
     k = teacher_idx.shape[-1]
@@ -99,14 +110,14 @@ def distill_loss_grad(ctx, logits, teacher_idx, teacher_logits, teacher_lse=None
         teacher_lse = _operand(ctx, teacher_lse, "teacher_lse", torch.float32, lead)
     if row_weight is not None:
         row_weight = _operand(ctx, row_weight, "row_weight", torch.float32, lead)
-    loss = torch.empty(lead, dtype=torch.float32, device=dev)
+    loss = _empty(lead, dtype=_f32, device=dev)
     grad, gstride = None, 0
     if want_grad:
-        grad = logits if in_place else torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        grad = logits if in_place else torch.empty_like(logits, memory_format=torch.contiguous_format)
         gstride = stride if in_place else vocab
     L._chk(ctx.lib.cbm_distill_loss_grad(ctx.h, logits.data_ptr(), dtype, rows, vocab, stride, teacher_idx.data_ptr(), teacher_logits.data_ptr(), k,
                                          _ptr(teacher_lse), _ptr(row_weight), temperature, loss.data_ptr(), _ptr(grad), gstride,
-                                         torch.cuda.current_stream(dev).cuda_stream))
+                                         _raw_stream(ctx.cfg.device)))
     return loss, grad
 
 
@@ -139,11 +150,11 @@ def verify_drafts(ctx, target_logits, draft_tokens, u_accept, u_sample, draft_lo
         if drafts == 0:
             draft_logits = None
     ws = _workspace(ctx.lib.cbm_verify_drafts_workspace(dtype, batch, drafts, vocab, draft_logits is not None, temperature), dev)
-    tokens = torch.empty(batch, positions, dtype=torch.int32, device=dev)
-    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
-    logprobs = torch.empty(batch, positions, dtype=torch.float32, device=dev)
+    tokens = _empty((batch, positions), dtype=_i32, device=dev)
+    accepted = _empty(batch, dtype=_i32, device=dev)
+    logprobs = _empty((batch, positions), dtype=_f32, device=dev)
     L._chk(ctx.lib.cbm_verify_drafts(ctx.h, target_logits.data_ptr(), dtype, batch, drafts, vocab, target_logits.stride(0), target_logits.stride(1),
                                      _ptr(draft_logits), dstride[0], dstride[1], _ptr(draft_tokens), _ptr(n_draft), _ptr(u_accept), _ptr(u_sample),
                                      temperature, tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(),
-                                     torch.cuda.current_stream(dev).cuda_stream))
+                                     _raw_stream(ctx.cfg.device)))
     return tokens, accepted, logprobs

@@ -372,6 +372,40 @@ def test_verify_rows_without_distribution(ctx, V):
         assert g[0][b].tolist() == tok and g[1][b] == a, (b, g[0][b], tok)
 
 
+@pytest.mark.parametrize("looked_up, ragged", [(False, True), (False, False), (True, True)])
+@pytest.mark.parametrize("dtype, B, K, V", [("bf16", 9, 8, 131072), ("f32", 500, 4, 4097), ("f16", 1, 33, 524288)])
+def test_verify_large_calls(ctx, dtype, B, K, V, looked_up, ragged):
+    """More than 2^24 logits: acceptance from fp32 sums, fp64 for the rows that tokens are drawn from."""
+    if looked_up and V == 4097:
+        B *= 2
+    rng = np.random.default_rng(B + V)
+    check_verify(ctx, *drafts_case(rng, B, K, V, dtype, 0.9, looked_up, ragged), 0.9)
+
+
+@pytest.mark.parametrize("looked_up", [False, True])
+def test_verify_a_batch_many_times(ctx, looked_up):
+    """The same sequences, some of them without a distribution somewhere, once and 40 times over (a large call): the same tokens, log-probabilities within both errors."""
+    rng = np.random.default_rng(3)
+    B, K, V = 10, 3, 9000
+    p, _, q, _, x, _, ua, us = drafts_case(rng, B, K, V, "f32", 1.0, False, False)
+    n = rng.integers(0, K + 1, B).astype(np.int32)
+    n[:6] = K
+    p[0, 0] = -math.inf
+    p[1, 1, 3] = math.nan
+    p[2, 3, 7] = math.inf
+    q[3, 0] = -math.inf
+    q[4, 1, 2] = math.nan
+    x[5, 0] = V
+    args = [cuda(a.astype(np.float32) if a.dtype == np.float64 else a) for a in (p, x, ua, us)]
+    tq, tn = None if looked_up else cuda(q.astype(np.float32)), cuda(n)
+    one = TK.verify_drafts(ctx, *args, draft_logits=tq, n_draft=tn)
+    R_ = 40 * (2 if looked_up else 1)
+    many = TK.verify_drafts(ctx, *[a.repeat(R_, *[1] * (a.dim() - 1)) for a in args], draft_logits=None if tq is None else tq.repeat(R_, 1, 1), n_draft=tn.repeat(R_))
+    for k in range(2):
+        assert torch.equal(one[k].repeat(R_, *[1] * (one[k].dim() - 1)), many[k])
+    assert (one[2].repeat(R_, 1) - many[2]).abs().max() <= 2 * D(V) + 4 * E * one[2].abs().max()
+
+
 def test_verify_extreme_random_numbers(ctx):
     """u = 0, the largest float below 1 and 1 itself (outside the range: still a token that has weight)."""
     V = 9001
@@ -510,3 +544,13 @@ def test_c_call_on_the_learner_stream_and_empty_calls(ctx):
     assert out.shape == (0, 3)
     with pytest.raises(L.CbmError, match="k 300"):
         TK.top_logits(ctx, torch.zeros(2, 400, device="cuda"), 300)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V, k", [(4000, 10), (40000, 33), (100000, 64), (70000, 100), (90000, 256)])
+def test_top_logits_overflowing_rows(ctx, dtype, V, k):
+    """Rows that keep beating the bar: rising in steps (many equal values each), the largest ones all in one thread's places, all equal but for a late few."""
+    up = np.arange(V)
+    z = np.stack([up // 50 / 64.0, up // 3000 * 1.0, np.where(up % 2048 < 8, 1.0 + up / V, 0.0), np.where(up % 8192 < 8, up // 8192, -1.0), np.where(up > V - 3, 2.0, 1.0), (up * 7919 % V) / V, up / V])
+    t = torch.as_tensor(z, dtype=torch.float32).to(DT[dtype])
+    check_top(ctx, t.double().numpy(), t.cuda(), k)
