@@ -91,22 +91,25 @@ template <int DT> __device__ __forceinline__ Pack tk_load(const char* row, int v
 __device__ __forceinline__ float tk_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float tk_base(float m) { return m == -INFINITY ? 0.0f : m; }   // what a maximum of -inf is replaced by: exp2(-inf - 0) = 0, not NaN
 
-// sum of 2^((z - b) c) over a pack, b >= every z.  One fma an element: 2^(z c - bc) with bc = fl(b c), what bc was rounded by goes into `fix` once a thread;
-// a maximum so large that b c might overflow takes the difference first.
+// 2^((z - b) c), b >= every z: one fma an element, 2^(z c - bc) with bc = fl(b c), what bc was rounded by goes into `fix`, a factor of the whole.  Where b c is so
+// large that this would not do (beyond 2^20: the roundings would be powers of two themselves), `far` says so, and exact differences are taken instead,
+// in rolled loops that read the row again: masks of a type's lowest values over whole rows come there, and little else.
 struct ExpSum {
   float b, c, bc, fix;
-  bool big;
-  __device__ __forceinline__ ExpSum(float base, float c_) : b(base), c(c_), bc(base * c_), big(fabsf(base) > 1e30f) { fix = big ? 1.0f : tk_exp2(-fmaf(base, c_, -bc)); }
-  template <int DT> __device__ __forceinline__ float usual(const Pack& x) const {
+  bool far;
+  __device__ __forceinline__ ExpSum(float base, float c_) : b(base), c(c_), bc(base * c_), fix(tk_exp2(-fmaf(base, c_, -bc))), far(!(fabsf(bc) <= 0x1p20f)) {}
+  __device__ __forceinline__ float operator()(float z) const { return tk_exp2(fmaf(z, c, -bc)); }
+  __device__ __forceinline__ float exact(float z) const { return tk_exp2((z - b) * c); }
+  template <int DT> __device__ __forceinline__ float sum(const Pack& x) const {
     float p = 0.0f;
 #pragma unroll
-    for (int j = 0; j < Lg<DT>::VEC; ++j) p += tk_exp2(fmaf(tk_get<DT>(x, j), c, -bc));
+    for (int j = 0; j < Lg<DT>::VEC; ++j) p += (*this)(tk_get<DT>(x, j));
     return p;
   }
-  template <int DT> __device__ __forceinline__ float large(const Pack& x) const {
+  template <int DT> __device__ __forceinline__ float exact_sum(const Pack& x) const {
     float p = 0.0f;
 #pragma unroll
-    for (int j = 0; j < Lg<DT>::VEC; ++j) p += tk_exp2((tk_get<DT>(x, j) - b) * c);
+    for (int j = 0; j < Lg<DT>::VEC; ++j) p += exact(tk_get<DT>(x, j));
     return p;
   }
 };
@@ -138,154 +141,153 @@ template <int T> __device__ __forceinline__ MS block_lse(float m, float s, float
 // s_T = sum of s outside the slots' tokens ("top"):
 //   loss  = w tau^2 [ sum_k t_k (log t_k - log s_{i_k}) + t_T (log t_T - log s_T) ]
 //   dz_j  = w tau   [ s_j (sum_k t_k + t_T) - sum_{k: i_k = j} t_k - [j outside top] t_T s_j / s_T ]
-// One block a row.  The row's first NV vectors a thread stay in registers, so that the logits are read once for statistics and gradient; what
-// lies behind them is read twice.  With a tail, a bitmap of the top tokens keeps them out of the streamed sum: s_T is then a sum of its own with
-// a maximum of its own, not a difference that cancels, and the top tokens join it from the wave that holds the teacher.  Every other token's
-// gradient is one coefficient times exp2((z - ref) c); the top tokens' gradients are stored last, over what the stream left there.
+// A block takes a row at a time.  The row's first NV vectors a thread stay in registers, so that the logits are read once for statistics and gradient;
+// what lies behind them is read twice.  With a tail, a bitmap of the top tokens keeps them out of the streamed sum: s_T is then a sum of its own with a maximum of its own, not a difference that cancels, and the top tokens join it from the wave that holds the
+// teacher.  Every other token's gradient is one coefficient times an exponential; the top tokens' gradients are stored last, over what the stream left.
+// log2(e) / tau is rounded to fp32 once and used so throughout the student's side, loss included: the loss of a temperature off by 6e-8.
 struct DistillArgs {
   const char* logits; int64_t ld;            // bytes from row to row
   char* grad; int64_t ldg;                   // null: loss only
   const int32_t* idx; const float* val; const float* lse; const float* weight;
   float* loss;
-  int V, K;
+  int rows, V, K;
   float c;                                   // log2(e) / tau
   double inv_tau, tau;
 };
+// a pack with the elements of `top` (a bit each) at -inf
+template <int DT> __device__ __forceinline__ void distill_mask(Pack& x, uint32_t top) {
+#pragma unroll
+  for (int j = 0; j < Lg<DT>::VEC; ++j) if (top >> j & 1) {
+    if constexpr (DT == CBM_F32) x.w[j] = TK_NEG<DT>;
+    else x.w[j >> 1] = j & 1 ? (x.w[j >> 1] & 0xffffu) | (TK_NEG<DT> & 0xffff0000u) : (x.w[j >> 1] & 0xffff0000u) | (TK_NEG<DT> & 0xffffu);
+  }
+}
+template <int DT> __device__ __forceinline__ Pack distill_pack(const Pack& x, const ExpSum& es, float coef) {
+  Pack g;
+#pragma unroll
+  for (int j = 0; j < Lg<DT>::VEC; j += 2) tk_put2<DT>(g, j, coef * es(tk_get<DT>(x, j)), coef * es(tk_get<DT>(x, j + 1)));
+  return g;
+}
+template <int DT> __device__ __forceinline__ Pack distill_pack_exact(const Pack& x, const ExpSum& es, float coef) {
+  Pack g;
+#pragma unroll
+  for (int j = 0; j < Lg<DT>::VEC; j += 2) tk_put2<DT>(g, j, coef * es.exact(tk_get<DT>(x, j)), coef * es.exact(tk_get<DT>(x, j + 1)));
+  return g;
+}
 template <int DT, int T, int NV, bool TAIL>
 __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
-  constexpr int VEC = Lg<DT>::VEC, ES = Lg<DT>::ES;
+  constexpr int VEC = Lg<DT>::VEC;
   __shared__ MS red[T / 64];
   __shared__ int32_t sidx[TK_MAX_TOP];
-  __shared__ float sz[TK_MAX_TOP];           // the student's logits at them
+  __shared__ float sz[TK_MAX_TOP], sv[TK_MAX_TOP];     // the student's and the teacher's logits there
   __shared__ double st[TK_MAX_TOP], slt[TK_MAX_TOP];   // t_k and log t_k
-  __shared__ bool sfirst[TK_MAX_TOP];        // whether a slot is the first one of its token
+  __shared__ uint8_t ssame[TK_MAX_TOP];      // 0: not the first slot of its token (or empty), 1: its only one, 2: the first of several
   __shared__ double steacher[2];             // sum of t_k, t_T
   __shared__ MS stop;                        // TAIL: (maximum, sum) of the student's logits at the top tokens
   extern __shared__ uint32_t bits[];         // TAIL: bit j set: token j is a top token
-  const int tid = threadIdx.x, V = a.V, K = a.K;
+  const int tid = threadIdx.x, V = a.V, K = a.K;   // (K <= T)
+  const int nfull = V / VEC, rem = V - nfull * VEC;
   const int64_t r = blockIdx.x;
   const char* row = a.logits + r * a.ld;
   char* grow = a.grad ? a.grad + r * a.ldg : nullptr;
   const float w = a.weight ? a.weight[r] : 1.0f;
-  const int nfull = V / VEC, rem = V - nfull * VEC;
-
-  const auto zeros = [&] {   // a row without a loss
+  const auto tops = [&](int v) { const int e = v * VEC; return bits[e >> 5] >> (e & 31) & ((1u << VEC) - 1); };
+  const auto zeros = [&] {                   // a row without a loss
     if (tid == 0) a.loss[r] = 0.0f;
     if (!grow) return;
     const Pack z = {{0, 0, 0, 0}};
     for (int v = tid; v < nfull; v += T) tk_store16(grow + (size_t)v * 16, z);
     if (tid < rem) tk_set<DT>(grow, nfull * VEC + tid, 0.0f);
   };
-  if (w == 0.0f) return zeros();   // padding: the row is not looked at
+  if (w == 0.0f) return zeros();             // padding: the row is not looked at
 
-  // the row, as far as it stays
-  Pack x[NV];
+  int my = -1;                               // slot `tid`: its token
+  float myv = -INFINITY, myz = -INFINITY;    // the teacher's and the student's logit
+  if (tid < K) {
+    my = a.idx[r * K + tid];
+    myv = a.val[r * K + tid];
+  }
+  Pack x[NV];                                // the row, as far as it stays; what lies behind its last whole vector is left out where it is used
+  if (nfull) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = i * T + tid;
-    x[i] = v < nfull ? tk_load16(row + (size_t)v * 16) : tk_neg<DT>();
+    for (int i = 0; i < NV; ++i) x[i] = tk_load16(row + (uint32_t)(min(i * T + tid, nfull - 1) * 16));
   }
-  const float xe = tid < rem ? tk_at<DT>(row, nfull * VEC + tid) : -INFINITY;   // the row's last few elements, one a thread
-
-  // the teacher's slots
-  int my = -1;
-  for (int k = tid; k < K; k += T) {
-    my = a.idx[r * K + k];
-    if ((uint32_t)my >= (uint32_t)V) my = -1;   // -1 and whatever lies outside the vocabulary: an empty slot
-    sidx[k] = my;
-    sz[k] = my >= 0 ? tk_at<DT>(row, my) : -INFINITY;
-  }
+  float xe = tid < rem ? tk_at<DT>(row, nfull * VEC + tid) : -INFINITY;   // the row's last few elements, one a thread
+  if ((uint32_t)my >= (uint32_t)V) my = -1;  // -1 and whatever lies outside the vocabulary: an empty slot
+  if (my >= 0) myz = tk_at<DT>(row, my);
+  if (tid < K) { sidx[tid] = my; sz[tid] = myz; sv[tid] = my >= 0 ? myv : -INFINITY; }
   if constexpr (TAIL) for (int i = tid; i < (V + 31) / 32; i += T) bits[i] = 0;
   __syncthreads();
-  for (int k = tid; k < K; k += T) {
-    const int t = sidx[k];
-    if constexpr (TAIL) if (t >= 0) atomicOr(&bits[t >> 5], 1u << (t & 31));
-    bool first = t >= 0;
-    for (int j = 0; j < k; ++j) first = first && sidx[j] != t;
-    sfirst[k] = first;
+  if (tid < K) {
+    int same = 0;
+    bool first = my >= 0;
+    for (int j = 0; j < K; ++j) if (sidx[j] == my) { ++same; first = first && j >= tid; }
+    ssame[tid] = !first ? 0 : (same == 1 ? 1 : 2);
+    if constexpr (TAIL) if (my >= 0) atomicOr(&bits[my >> 5], 1u << (my & 31));
   }
-  if (tid < 64) {                             // t_k in fp64: a few exps, under the row's loads
-    float v[TK_MAX_TOP / 64];
+  if constexpr (TAIL) __syncthreads();
+  if (tid < 64) {                        // t_k in fp64, and the top tokens' own (maximum, sum), each token once: beside the other waves' statistics
     float vm = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < TK_MAX_TOP / 64; ++q) {
-      const int k = q * 64 + tid;
-      v[q] = k < K && sidx[k] >= 0 ? a.val[r * K + k] : -INFINITY;
-      vm = fmaxf(vm, v[q]);
-    }
-    double lt[TK_MAX_TOP / 64], t[TK_MAX_TOP / 64], sum = 0.0;
-    const double ref = TAIL ? (double)a.lse[r] : (double)tk_base(wave_max(vm)) * a.inv_tau;
-#pragma unroll
-    for (int q = 0; q < TK_MAX_TOP / 64; ++q) {
-      lt[q] = (double)v[q] * a.inv_tau - ref;
-      t[q] = v[q] == -INFINITY ? 0.0 : exp(lt[q]);
-      sum += t[q];
+    for (int k = tid; k < K; k += 64) vm = fmaxf(vm, sv[k]);
+    const double at = TAIL ? (double)a.lse[r] : (double)tk_base(wave_max(vm)) * a.inv_tau;
+    double sum = 0.0;
+    for (int k = tid; k < K; k += 64) {
+      const double lt = (double)sv[k] * a.inv_tau - at, t = sv[k] == -INFINITY ? 0.0 : exp(lt);
+      st[k] = t; slt[k] = lt;
+      sum += t;
     }
     sum = wave_sum(sum);
-    const double logsum = TAIL || !(sum > 0.0) ? 0.0 : log(sum), scale = TAIL || !(sum > 0.0) ? 1.0 : 1.0 / sum;
-#pragma unroll
-    for (int q = 0; q < TK_MAX_TOP / 64; ++q) if (q * 64 + tid < K) { st[q * 64 + tid] = t[q] * scale; slt[q * 64 + tid] = lt[q] - logsum; }
-    if (tid == 0) {
-      steacher[0] = !TAIL && sum > 0.0 ? 1.0 : sum;
-      steacher[1] = TAIL ? (sum > 1.0 ? 0.0 : 1.0 - sum) : 0.0;
+    if (!TAIL && sum > 0.0) {
+      const double ls = log(sum), inv = 1.0 / sum;
+      for (int k = tid; k < K; k += 64) { st[k] *= inv; slt[k] -= ls; }
+      sum = 1.0;
+    }
+    if (tid == 0) { steacher[0] = sum; steacher[1] = TAIL ? (sum > 1.0 ? 0.0 : 1.0 - sum) : 0.0; }
+    if constexpr (TAIL) {
+      float zm = -INFINITY;
+      for (int k = tid; k < K; k += 64) if (ssame[k]) zm = fmaxf(zm, sz[k]);
+      zm = wave_max(zm);
+      double zs = 0.0;
+      for (int k = tid; k < K; k += 64) if (ssame[k]) zs += (double)tk_exp2((sz[k] - tk_base(zm)) * a.c);
+      zs = wave_sum(zs);
+      if (tid == 0) stop = MS{zm, zs};
     }
   }
-  __syncthreads();
-  if constexpr (TAIL) if (tid < 64) {         // the top tokens' own (maximum, sum), each token once
-    float m = -INFINITY;
-    for (int k = tid; k < K; k += 64) if (sfirst[k]) m = fmaxf(m, sz[k]);
-    m = wave_max(m);
-    double s = 0.0;
-    for (int k = tid; k < K; k += 64) if (sfirst[k]) s += (double)tk_exp2((sz[k] - tk_base(m)) * a.c);
-    s = wave_sum(s);
-    if (tid == 0) stop = MS{m, s};
-  }
-
   // statistics of the row (TAIL: of what lies outside top)
   float m = xe;
-  if constexpr (TAIL) { if (tid < rem) { const int e = nfull * VEC + tid; if (bits[e >> 5] >> (e & 31) & 1) m = -INFINITY; } }
+  if constexpr (TAIL) if (tid < rem) { const int e = nfull * VEC + tid; if (bits[e >> 5] >> (e & 31) & 1) m = -INFINITY; }
   const float xs = m;
+  int t = cbm_opaque_vgpr(tid);          // (or the compiler keeps NV places and masks from pass to pass, in registers that the row needs)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if constexpr (TAIL) {
-      const int v = i * T + tid, e = v * VEC;
-      const uint32_t top = v < nfull ? bits[e >> 5] >> (e & 31) & ((1u << VEC) - 1) : 0u;
-      if (top) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) if (top >> j & 1) {
-          if constexpr (ES == 4) x[i].w[j] = TK_NEG<DT>;
-          else x[i].w[j >> 1] = j & 1 ? (x[i].w[j >> 1] & 0xffffu) | (TK_NEG<DT> & 0xffff0000u) : (x[i].w[j >> 1] & 0xffff0000u) | (TK_NEG<DT> & 0xffffu);
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) m = fmaxf(m, tk_get<DT>(x[i], j));
-  }
-  float s = tk_exp2((xs - tk_base(m)) * a.c);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
+    const int v = i * T + t;
+    if constexpr (TAIL) { const uint32_t top = tops(max(min(v, nfull - 1), 0)); if (top) distill_mask<DT>(x[i], top); }
+    const float vm = tk_max<DT>(x[i]);
+    m = v < nfull ? fmaxf(m, vm) : m;
     tk_redecode(x[i]);
-    float p = 0.0f;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) p += tk_exp2((tk_get<DT>(x[i], j) - tk_base(m)) * a.c);
-    s += p;
   }
-  for (int v = NV * T + tid; v < nfull; v += T) {   // what does not stay: running maximum and sum
-    const Pack y = tk_load16(row + (size_t)v * 16);
-    uint32_t top = 0;
-    if constexpr (TAIL) { const int e = v * VEC; top = bits[e >> 5] >> (e & 31) & ((1u << VEC) - 1); }
-    float z[VEC], nm = m;
+  const ExpSum es(tk_base(m), a.c);
+  float s = tk_exp2((xs - es.b) * a.c), p = 0.0f;
+  t = cbm_opaque_vgpr(tid);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) { z[j] = top >> j & 1 ? -INFINITY : tk_get<DT>(y, j); nm = fmaxf(nm, z[j]); }
-    const float b = tk_base(nm);
-    float p = 0.0f;
+  for (int i = 0; i < NV; ++i) {
+    const float q = es.sum<DT>(x[i]);
+    p += i * T + t < nfull ? q : 0.0f;
+    tk_redecode(x[i]);
+  }
+  s += es.far ? 0.0f : p * es.fix;
+  for (int v = (es.far ? 0 : NV * T) + tid; v < nfull; v += T) {   // what does not stay: running maximum and sum
+    Pack y = tk_load16(row + (size_t)v * 16);
+    if constexpr (TAIL) { const uint32_t top = tops(v); if (top) distill_mask<DT>(y, top); }
+    const float nm = fmaxf(m, tk_max<DT>(y)), b = tk_base(nm);
+    float q = 0.0f;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) p += tk_exp2((z[j] - b) * a.c);
-    s = s * tk_exp2((m - b) * a.c) + p;
+    for (int j = 0; j < VEC; ++j) q += tk_exp2((tk_get<DT>(y, j) - b) * a.c);
+    s = s * tk_exp2((m - b) * a.c) + q;
     m = nm;
   }
   const MS ms = block_lse<T>(m, s, a.c, red);
-  if constexpr (T == 64) __syncthreads();   // (stop; a wider block has passed one in block_lse)
+  if constexpr (T == 64) __syncthreads();   // (a wider block has passed one in block_lse)
   // the whole row's statistics, and the coefficient of the tokens outside top
   float M = ms.m;
   double S = ms.s, tT = 0.0;
@@ -296,14 +298,14 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
     S = ms.s * (double)tk_exp2((ms.m - B) * a.c) + stop.s * (double)tk_exp2((stop.m - B) * a.c);
     tT = ms.m == -INFINITY ? 0.0 : steacher[1];   // no logit outside top: the tail is left out
   }
-  if (S == 0.0 || (!TAIL && sumT == 0.0)) return zeros();   // nothing in the student's row, or nothing in the teacher's (S, sumT: the same for every thread)
+  if (S == 0.0 || (!TAIL && sumT == 0.0)) return zeros();   // nothing in the student's row, or nothing in the teacher's (the same for every thread)
   if (tid < 64) {
-    const double logS = log(S);
+    const double logS = log(S), lc = (double)a.c * 0.69314718055994530942;
     double l = 0.0;
-    for (int k = tid; k < K; k += 64) if (st[k] != 0.0) l += st[k] * (slt[k] - (((double)sz[k] - (double)M) * a.inv_tau - logS));
+    for (int k = tid; k < K; k += 64) if (st[k] != 0.0) l += st[k] * (slt[k] - (((double)sz[k] - (double)M) * lc - logS));
     l = wave_sum(l);
     if (tid == 0) {
-      if (tT > 0.0) l += tT * (log(tT) - (((double)ms.m - (double)M) * a.inv_tau + log(ms.s) - logS));
+      if (tT > 0.0) l += tT * (log(tT) - (((double)ms.m - (double)M) * lc + log(ms.s) - logS));
       a.loss[r] = (float)((double)w * a.tau * a.tau * l);
     }
   }
@@ -311,57 +313,50 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   const double wt = (double)w * a.tau;
   float ref, coef;
   if constexpr (TAIL) {
-    ref = tk_base(ms.m);   // exp2((z - ref) c) <= 1 for every token outside top
+    ref = tk_base(ms.m);                     // 2^((z - ref) c) <= 1 for every token outside top
     const double sT = ms.s * (double)tk_exp2((ms.m - tk_base(M)) * a.c) / S;   // their probability
     coef = ms.m == -INFINITY ? 0.0f : (float)(wt * ((sumT + tT) * sT - tT) / ms.s);
   } else {
     ref = tk_base(M);
     coef = (float)(wt * sumT / S);
   }
-  // (an infinite exp2 of a top token is overwritten below; a NaN in the row has made coef NaN)
+  // (an infinite 2^.. of a top token is overwritten below; a NaN in the row has made coef NaN)
+  const ExpSum eg(ref, a.c);
+  if (!eg.far) {
+    const float cf = coef * eg.fix;
+    t = cbm_opaque_vgpr(tid);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = i * T + tid;
-    if (v < nfull) {
+    for (int i = 0; i < NV; ++i) {
       tk_redecode(x[i]);
-      Pack g;
-#pragma unroll
-      for (int j = 0; j < VEC; j += 2) tk_put2<DT>(g, j, coef * tk_exp2((tk_get<DT>(x[i], j) - ref) * a.c), coef * tk_exp2((tk_get<DT>(x[i], j + 1) - ref) * a.c));
-      tk_store16(grow + (size_t)v * 16, g);
+      const Pack g = distill_pack<DT>(x[i], eg, cf);
+      if (i * T + t < nfull) tk_store16(grow + (uint32_t)((i * T + t) * 16), g);
     }
   }
-  for (int v = NV * T + tid; v < nfull; v += T) {
-    const Pack y = tk_load16(row + (size_t)v * 16);
-    Pack g;
-#pragma unroll
-    for (int j = 0; j < VEC; j += 2) tk_put2<DT>(g, j, coef * tk_exp2((tk_get<DT>(y, j) - ref) * a.c), coef * tk_exp2((tk_get<DT>(y, j + 1) - ref) * a.c));
-    tk_store16(grow + (size_t)v * 16, g);
-  }
-  if (tid < rem) tk_set<DT>(grow, nfull * VEC + tid, coef * tk_exp2((xe - ref) * a.c));
-  __syncthreads();   // the stream's stores come before the top tokens'
-  for (int k = tid; k < K; k += T) {
-    if (!sfirst[k]) continue;
-    const int t = sidx[k];
-    double d = 0.0;
-    for (int j = k; j < K; ++j) if (sidx[j] == t) d += st[j];   // a token in several slots: all of their t_k
-    const double sk = (double)tk_exp2((sz[k] - tk_base(M)) * a.c) / S;
-    tk_set<DT>(grow, t, (float)(wt * (sk * (sumT + tT) - d)));
+  for (int v = (eg.far ? 0 : NV * T) + tid; v < nfull; v += T) tk_store16(grow + (size_t)v * 16, distill_pack_exact<DT>(tk_load16(row + (size_t)v * 16), eg, coef));
+  if (tid < rem) tk_set<DT>(grow, nfull * VEC + tid, coef * eg.exact(xe));
+  __syncthreads();                           // the stream's stores come before the top tokens'
+  if (tid < K && ssame[tid]) {
+    double d = st[tid];
+    if (ssame[tid] == 2) for (int j = tid + 1; j < K; ++j) if (sidx[j] == my) d += st[j];   // a token in several slots: all of their t_k
+    const double sk = (double)tk_exp2((myz - tk_base(M)) * a.c) / S;
+    tk_set<DT>(grow, my, (float)(wt * (sk * (sumT + tT) - d)));
   }
 }
 
 template <int DT, int T, int NV>
-void distill_launch(const DistillArgs& a, int rows, hipStream_t st) {
-  if (a.lse) hipLaunchKernelGGL((distill_kernel<DT, T, NV, true>), dim3(rows), dim3(T), ((a.V + 31) / 32) * 4, st, a);
-  else hipLaunchKernelGGL((distill_kernel<DT, T, NV, false>), dim3(rows), dim3(T), 0, st, a);
+void distill_launch(const DistillArgs& a, hipStream_t st) {
+  if (a.lse) hipLaunchKernelGGL((distill_kernel<DT, T, NV, true>), dim3(a.rows), dim3(T), ((a.V + 31) / 32) * 4, st, a);
+  else hipLaunchKernelGGL((distill_kernel<DT, T, NV, false>), dim3(a.rows), dim3(T), 0, st, a);
 }
-// the smallest block and register tile that hold the row (a wave holds K slots' threads up to 64); a row beyond 1024 x 16 vectors (256 KB) is held as far as that goes
+// the smallest block and register tile that hold the row; a row beyond 1024 x 16 vectors (256 KB) is held as far as that goes.  K <= T.
 template <int DT>
-void distill_dispatch(const DistillArgs& a, int rows, hipStream_t st) {
+void distill_dispatch(const DistillArgs& a, hipStream_t st) {
   const int nv = (a.V + Lg<DT>::VEC - 1) / Lg<DT>::VEC;
-  if (nv <= 64) distill_launch<DT, 64, 1>(a, rows, st);
-  else if (nv <= 4 * 256) distill_launch<DT, 256, 4>(a, rows, st);
-  else if (nv <= 16 * 256) distill_launch<DT, 256, 16>(a, rows, st);
-  else distill_launch<DT, 1024, 16>(a, rows, st);
+  if (nv <= 64 && a.K <= 64) distill_launch<DT, 64, 1>(a, st);
+  else if (nv <= 4 * 256) distill_launch<DT, 256, 4>(a, st);
+  else if (nv <= 16 * 256) distill_launch<DT, 256, 16>(a, st);
+  else if (nv <= 16 * 512) distill_launch<DT, 512, 16>(a, st);
+  else distill_launch<DT, 1024, 16>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------ the K largest logits of a row
@@ -510,18 +505,17 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
     const float nm = fmaxf(m, cm);
     const ExpSum es(tk_base(nm), a.c);
     float p = 0.0f;
-    if (!es.big) {
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int u = 0; u < U; ++u) { p += es.usual<DT>(x[g][u]); tk_redecode(x[g][u]); }
-    } else {
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int u = 0; u < U; ++u) { p += es.large<DT>(x[g][u]); tk_redecode(x[g][u]); }
+      for (int u = 0; u < U; ++u) { p += es.sum<DT>(x[g][u]); tk_redecode(x[g][u]); }
+    p *= es.fix;
+    if (es.far) {
+      p = 0.0f;
+#pragma unroll 1
+      for (int q = 0; q < G * U; ++q) { const int v = (c * U + q) * T + tid; if (c + q / U < c1 && v < nfull) p += es.exact_sum<DT>(tk_load16(row + (size_t)v * 16)); }
     }
-    s = s * tk_exp2((m - es.b) * a.c) + p * es.fix;
+    s = s * tk_exp2((m - es.b) * a.c) + p;
     m = nm;
     float over = bar;                        // what an element of this group has to be above: just below the bar while equal ones may come before those that made it
     if (c == c0) {
@@ -798,14 +792,15 @@ __global__ __launch_bounds__(VF_T) void verify_stats_kernel(VerifyArgs a) {
     for (int u = 0; u < U; ++u) { nm = fmaxf(nm, tk_max<DT>(x[u])); tk_redecode(x[u]); }
     const ExpSum es(tk_base(nm), a.c);
     float p = 0.0f;
-    if (!es.big) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) p += es.usual<DT>(x[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) p += es.large<DT>(x[u]);
+    for (int u = 0; u < U; ++u) p += es.sum<DT>(x[u]);
+    p *= es.fix;
+    if (es.far) {
+      p = 0.0f;
+#pragma unroll 1
+      for (int u = 0; u < U; ++u) { const int at = v + u * VF_T + (int)threadIdx.x; if (at < v1) p += es.exact_sum<DT>(tk_load<DT>(z, at, a.V)); }
     }
-    s = s * tk_exp2((m - es.b) * a.c) + p * es.fix;
+    s = s * tk_exp2((m - es.b) * a.c) + p;
     m = nm;
   }
   const MS ms = block_lse<VF_T>(m, s, a.c, red);
@@ -1318,12 +1313,12 @@ extern "C" int cbm_distill_loss_grad(cbm_ctx* c, const void* logits, int32_t dty
   a.logits = (const char*)logits; a.ld = row_stride * es;
   a.grad = (char*)dlogits; a.ldg = grad_stride * es;
   a.idx = teacher_idx; a.val = teacher_logits; a.lse = teacher_lse; a.weight = row_weight; a.loss = loss;
-  a.V = vocab; a.K = k;
+  a.rows = rows; a.V = vocab; a.K = k;
   a.tau = (double)temperature; a.inv_tau = 1.0 / a.tau; a.c = (float)(TK_LOG2E * a.inv_tau);
   hipStream_t st = tk_stream(c, stream);
-  if (dtype == CBM_F32) distill_dispatch<CBM_F32>(a, rows, st);
-  else if (dtype == CBM_BF16) distill_dispatch<CBM_BF16>(a, rows, st);
-  else distill_dispatch<CBM_F16>(a, rows, st);
+  if (dtype == CBM_F32) distill_dispatch<CBM_F32>(a, st);
+  else if (dtype == CBM_BF16) distill_dispatch<CBM_BF16>(a, st);
+  else distill_dispatch<CBM_F16>(a, st);
   return tk_done(fn);
 }
 
