@@ -176,7 +176,7 @@ template <int DT> __device__ __forceinline__ Pack distill_pack_exact(const Pack&
 }
 template <int DT, int T, int NV, bool TAIL>
 __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
-  constexpr int VEC = Lg<DT>::VEC;
+  constexpr int VEC = Lg<DT>::VEC, ES = Lg<DT>::ES, U = 4;
   __shared__ MS red[T / 64];
   __shared__ int32_t sidx[TK_MAX_TOP];
   __shared__ float sz[TK_MAX_TOP], sv[TK_MAX_TOP];     // the student's and the teacher's logits there
@@ -186,18 +186,25 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   __shared__ MS stop;                        // TAIL: (maximum, sum) of the student's logits at the top tokens
   extern __shared__ uint32_t bits[];         // TAIL: bit j set: token j is a top token
   const int tid = threadIdx.x, V = a.V, K = a.K;   // (K <= T)
-  const int nfull = V / VEC, rem = V - nfull * VEC;
   const int64_t r = blockIdx.x;
-  const char* row = a.logits + r * a.ld;
-  char* grow = a.grad ? a.grad + r * a.ldg : nullptr;
+  // The row's vectors begin where 16 bytes do (a row of an odd vocabulary starts anywhere); the up to VEC - 1 elements before and behind them are one a thread.
+  const char* row0 = a.logits + r * a.ld;
+  char* grow0 = a.grad ? a.grad + r * a.ldg : nullptr;
+  const int head = min((int)(-(uintptr_t)row0 & 15) / ES, V), nfull = (V - head) / VEC, rem = V - nfull * VEC;
+  const char* row = row0 + head * ES;
+  char* grow = grow0 + head * ES;
+  const int ee = tid < head ? tid : nfull * VEC + tid;   // the thread's single element, where tid < rem
   const float w = a.weight ? a.weight[r] : 1.0f;
-  const auto tops = [&](int v) { const int e = v * VEC; return bits[e >> 5] >> (e & 31) & ((1u << VEC) - 1); };
+  const auto tops = [&](int v) {             // the bits of vector v's elements
+    const int e = head + v * VEC;
+    return (uint32_t)((((uint64_t)bits[(e >> 5) + 1] << 32) | bits[e >> 5]) >> (e & 31)) & ((1u << VEC) - 1);
+  };
   const auto zeros = [&] {                   // a row without a loss
     if (tid == 0) a.loss[r] = 0.0f;
-    if (!grow) return;
+    if (!grow0) return;
     const Pack z = {{0, 0, 0, 0}};
     for (int v = tid; v < nfull; v += T) tk_store16(grow + (size_t)v * 16, z);
-    if (tid < rem) tk_set<DT>(grow, nfull * VEC + tid, 0.0f);
+    if (tid < rem) tk_set<DT>(grow0, ee, 0.0f);
   };
   if (w == 0.0f) return zeros();             // padding: the row is not looked at
 
@@ -210,13 +217,13 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   Pack x[NV];                                // the row, as far as it stays; what lies behind its last whole vector is left out where it is used
   if (nfull) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = tk_load16(row + (uint32_t)(min(i * T + tid, nfull - 1) * 16));
+    for (int i = 0; i < NV; ++i) if (i * T < nfull) x[i] = tk_load16(row + (uint32_t)(min(i * T + tid, nfull - 1) * 16));
   }
-  float xe = tid < rem ? tk_at<DT>(row, nfull * VEC + tid) : -INFINITY;   // the row's last few elements, one a thread
+  const float xe = tid < rem ? tk_at<DT>(row0, ee) : -INFINITY;
   if ((uint32_t)my >= (uint32_t)V) my = -1;  // -1 and whatever lies outside the vocabulary: an empty slot
-  if (my >= 0) myz = tk_at<DT>(row, my);
+  if (my >= 0) myz = tk_at<DT>(row0, my);
   if (tid < K) { sidx[tid] = my; sz[tid] = myz; sv[tid] = my >= 0 ? myv : -INFINITY; }
-  if constexpr (TAIL) for (int i = tid; i < (V + 31) / 32; i += T) bits[i] = 0;
+  if constexpr (TAIL) for (int i = tid; i < (V + 31) / 32 + 1; i += T) bits[i] = 0;
   __syncthreads();
   if (tid < K) {
     int same = 0;
@@ -255,11 +262,12 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   }
   // statistics of the row (TAIL: of what lies outside top)
   float m = xe;
-  if constexpr (TAIL) if (tid < rem) { const int e = nfull * VEC + tid; if (bits[e >> 5] >> (e & 31) & 1) m = -INFINITY; }
+  if constexpr (TAIL) if (tid < rem) { if (bits[ee >> 5] >> (ee & 31) & 1) m = -INFINITY; }
   const float xs = m;
   int t = cbm_opaque_vgpr(tid);          // (or the compiler keeps NV places and masks from pass to pass, in registers that the row needs)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    if (i * T >= nfull) continue;            // (the same for every thread)
     const int v = i * T + t;
     if constexpr (TAIL) { const uint32_t top = tops(max(min(v, nfull - 1), 0)); if (top) distill_mask<DT>(x[i], top); }
     const float vm = tk_max<DT>(x[i]);
@@ -271,19 +279,36 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   t = cbm_opaque_vgpr(tid);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    if (i * T >= nfull) continue;
     const float q = es.sum<DT>(x[i]);
     p += i * T + t < nfull ? q : 0.0f;
     tk_redecode(x[i]);
   }
   s += es.far ? 0.0f : p * es.fix;
-  for (int v = (es.far ? 0 : NV * T) + tid; v < nfull; v += T) {   // what does not stay: running maximum and sum
-    Pack y = tk_load16(row + (size_t)v * 16);
-    if constexpr (TAIL) { const uint32_t top = tops(v); if (top) distill_mask<DT>(y, top); }
-    const float nm = fmaxf(m, tk_max<DT>(y)), b = tk_base(nm);
-    float q = 0.0f;
+  for (int v0 = (es.far ? 0 : NV * T) + tid; v0 < nfull; v0 += U * T) {   // what does not stay: running maximum and sum, U vectors in flight
+    Pack y[U];
+    float nm = m;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) q += tk_exp2((tk_get<DT>(y, j) - b) * a.c);
-    s = s * tk_exp2((m - b) * a.c) + q;
+    for (int u = 0; u < U; ++u) y[u] = tk_load16(row + (uint32_t)(min(v0 + u * T, nfull - 1) * 16));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * T;
+      if constexpr (TAIL) { const uint32_t top = tops(min(v, nfull - 1)); if (top) distill_mask<DT>(y[u], top); }
+      const float vm = tk_max<DT>(y[u]);
+      nm = v < nfull ? fmaxf(nm, vm) : nm;
+      tk_redecode(y[u]);
+    }
+    const ExpSum ey(tk_base(nm), a.c);
+    float q = 0.0f;
+    if (!ey.far) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) { const float e = ey.sum<DT>(y[u]); q += v0 + u * T < nfull ? e : 0.0f; }
+      q *= ey.fix;
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) { const float e = ey.exact_sum<DT>(y[u]); q += v0 + u * T < nfull ? e : 0.0f; }
+    }
+    s = s * tk_exp2((m - ey.b) * a.c) + q;
     m = nm;
   }
   const MS ms = block_lse<T>(m, s, a.c, red);
@@ -309,7 +334,7 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
       a.loss[r] = (float)((double)w * a.tau * a.tau * l);
     }
   }
-  if (!grow) return;
+  if (!grow0) return;
   const double wt = (double)w * a.tau;
   float ref, coef;
   if constexpr (TAIL) {
@@ -327,36 +352,48 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
     t = cbm_opaque_vgpr(tid);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (i * T >= nfull) continue;
       tk_redecode(x[i]);
       const Pack g = distill_pack<DT>(x[i], eg, cf);
       if (i * T + t < nfull) tk_store16(grow + (uint32_t)((i * T + t) * 16), g);
     }
   }
-  for (int v = (eg.far ? 0 : NV * T) + tid; v < nfull; v += T) tk_store16(grow + (size_t)v * 16, distill_pack_exact<DT>(tk_load16(row + (size_t)v * 16), eg, coef));
-  if (tid < rem) tk_set<DT>(grow, nfull * VEC + tid, coef * eg.exact(xe));
+  for (int v0 = (eg.far ? 0 : NV * T) + tid; v0 < nfull; v0 += U * T) {
+    Pack y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) y[u] = tk_load16(row + (uint32_t)(min(v0 + u * T, nfull - 1) * 16));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Pack g = eg.far ? distill_pack_exact<DT>(y[u], eg, coef) : distill_pack<DT>(y[u], eg, coef * eg.fix);
+      if (v0 + u * T < nfull) tk_store16(grow + (uint32_t)((v0 + u * T) * 16), g);
+    }
+  }
+  if (tid < rem) tk_set<DT>(grow0, ee, coef * eg.exact(xe));
   __syncthreads();                           // the stream's stores come before the top tokens'
   if (tid < K && ssame[tid]) {
     double d = st[tid];
     if (ssame[tid] == 2) for (int j = tid + 1; j < K; ++j) if (sidx[j] == my) d += st[j];   // a token in several slots: all of their t_k
     const double sk = (double)tk_exp2((myz - tk_base(M)) * a.c) / S;
-    tk_set<DT>(grow, my, (float)(wt * (sk * (sumT + tT) - d)));
+    tk_set<DT>(grow0, my, (float)(wt * (sk * (sumT + tT) - d)));
   }
 }
 
 template <int DT, int T, int NV>
 void distill_launch(const DistillArgs& a, hipStream_t st) {
-  if (a.lse) hipLaunchKernelGGL((distill_kernel<DT, T, NV, true>), dim3(a.rows), dim3(T), ((a.V + 31) / 32) * 4, st, a);
+  if (a.lse) hipLaunchKernelGGL((distill_kernel<DT, T, NV, true>), dim3(a.rows), dim3(T), ((a.V + 31) / 32 + 1) * 4, st, a);
   else hipLaunchKernelGGL((distill_kernel<DT, T, NV, false>), dim3(a.rows), dim3(T), 0, st, a);
 }
-// the smallest block and register tile that hold the row; a row beyond 1024 x 16 vectors (256 KB) is held as far as that goes.  K <= T.
+// 8 vectors a thread stay; a block of 256, 512 or 1024 threads has 6, 3 or 1.5 others beside it on its compute unit, whose loads, sums and stores overlap its
+// own.  A larger block reads less of its row twice, a smaller one has more company.  3840 rows with gradient, us by blocks of 256 / 512 / 1024:
+// 20000 bf16 (2500 vectors) 70 / 86 / 144, 32768 bf16 122 / 106 / 170, 65536 bf16 (8192) 260 / 216 / 251, 50021 fp32 (12506) 453 / 358 / 325,
+// 131072 bf16 (16384) 575 / 470 / 427.  16 vectors a thread: 431 there, 200 against 140 at 40000 bf16 (two blocks of 150 registers do not fit).  K <= T.
 template <int DT>
 void distill_dispatch(const DistillArgs& a, hipStream_t st) {
   const int nv = (a.V + Lg<DT>::VEC - 1) / Lg<DT>::VEC;
   if (nv <= 64 && a.K <= 64) distill_launch<DT, 64, 1>(a, st);
-  else if (nv <= 4 * 256) distill_launch<DT, 256, 4>(a, st);
-  else if (nv <= 16 * 256) distill_launch<DT, 256, 16>(a, st);
-  else if (nv <= 16 * 512) distill_launch<DT, 512, 16>(a, st);
-  else distill_launch<DT, 1024, 16>(a, st);
+  else if (nv <= 10 * 256) distill_launch<DT, 256, 8>(a, st);
+  else if (nv <= 20 * 512) distill_launch<DT, 512, 8>(a, st);
+  else distill_launch<DT, 1024, 8>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------ the K largest logits of a row
@@ -479,10 +516,13 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
   const int tid = threadIdx.x, V = a.V, K = a.K;
   const int64_t r = blockIdx.x / (uint32_t)a.nsplit;
   const int split = (int)(blockIdx.x - r * a.nsplit);
-  const char* row = a.logits + r * a.ld;
-  const int nfull = V / VEC, rem = V - nfull * VEC, nchunk = (nfull + T * U - 1) / (T * U);   // (V > 64: there are whole vectors)
+  // the row's vectors begin where 16 bytes do; the up to VEC - 1 elements before and behind them are one a thread of the last split
+  const char* row0 = a.logits + r * a.ld;
+  const int head = (int)(-(uintptr_t)row0 & 15) / Lg<DT>::ES, nfull = (V - head) / VEC, rem = V - nfull * VEC, nchunk = (nfull + T * U - 1) / (T * U);   // (V > 64: there are whole vectors)
+  const char* row = row0 + head * Lg<DT>::ES;
   const int c0 = (int)((int64_t)nchunk * split / a.nsplit), c1 = (int)((int64_t)nchunk * (split + 1) / a.nsplit);
-  const float extra = split == a.nsplit - 1 && tid < rem ? tk_at<DT>(row, nfull * VEC + tid) : -INFINITY;   // the row's last few elements, one a thread
+  const int ee = tid < head ? tid : nfull * VEC + tid;
+  const float extra = split == a.nsplit - 1 && tid < rem ? tk_at<DT>(row0, ee) : -INFINITY;
   Pack x[G][U];                              // G chunks at a time: one bar, one maximum, one rescaling for all; each chunk's registers take the next group's as it is done
 #pragma unroll
   for (int g = 0; g < G; ++g) top_chunk<DT, T, U>(x[g], row, c0 + g < c1 ? c0 + g : nchunk, nfull);
@@ -542,7 +582,7 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
       for (uint32_t w = waits; w; w &= w - 1) {
         const int q = __builtin_ctz(w), e = ((ch * U + q / VEC) * T + tid) * VEC + q % VEC;
         const float z = tk_at<DT>(row, e);
-        const uint64_t k = top_key(z, e);
+        const uint64_t k = top_key(z, head + e);
         if (z > over && k >= bound) {
           const int at = atomicAdd(&sh.fill, 1);
           if (at < a.cap) buf[at] = k;
@@ -576,7 +616,7 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
         for (uint32_t v = w; v; v &= v - 1) {
           const int q = __builtin_ctz(v), e = (((c + g) * U + q / VEC) * T + tid) * VEC + q % VEC;
           const float z = tk_at<DT>(row, e);
-          const uint64_t k = top_key(z, e);
+          const uint64_t k = top_key(z, head + e);
           if (z > over && k > best) best = k;
         }
         const uint64_t bound = top_bound<T, uint64_t>(best, TOP_KEY_BITS, K, 0, sh.all, &sh.bound);   // (0: fewer than K threads wait, all they hold fits)
@@ -598,7 +638,7 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
   __syncthreads();
   fill = top_cut<T, EPT>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
   if (rem && split == a.nsplit - 1) {        // (cap has room for EPT K more than T)
-    if (extra > bar) buf[atomicAdd(&sh.fill, 1)] = top_key(extra, nfull * VEC + tid);
+    if (extra > -INFINITY && extra >= bar) buf[atomicAdd(&sh.fill, 1)] = top_key(extra, ee);   // (those before the vectors count where they equal the bar)
     __syncthreads();
     fill = sh.fill;
     __syncthreads();

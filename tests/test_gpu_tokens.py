@@ -252,7 +252,7 @@ def test_distill_poison_and_padding(ctx):
             beside[off:off + V] = False
             assert buf[:, beside].isnan().all()
             view.copy_(t)
-            _, g = TK.distill_loss_grad(ctx, t, cuda(idx.astype(np.int32)), cuda(v.astype(np.float32)), row_weight=cuda(w.astype(np.float32)))
+            _, g = TK.distill_loss_grad(ctx, view, cuda(idx.astype(np.int32)), cuda(v.astype(np.float32)), row_weight=cuda(w.astype(np.float32)))   # (at these addresses: the order of a row's sum goes by its alignment)
             TK.distill_loss_grad(ctx, view, cuda(idx.astype(np.int32)), cuda(v.astype(np.float32)), row_weight=cuda(w.astype(np.float32)), in_place=True)
             assert torch.equal(g, view)
 
