@@ -400,7 +400,7 @@ void distill_dispatch(const DistillArgs& a, hipStream_t st) {
 // Keys: (order of the fp32 value, 19 bits of 2^19 - 1 - index): unique, and their order is "larger value first, equal values by rising index".
 // A block streams its row (or its share of one: few rows are split and joined) in chunks of EPT elements a thread, with the running maximum and
 // sum a thread for the log-sum-exp, and appends what is above a bar to a buffer in LDS.  The first bar comes from the first chunk: the K-th largest
-// of the threads' maxima has K elements at or above it, and with T >= 4 K threads few more (1.2 K of random data).  After the 2nd, 4th, 8th .. chunk the
+// of the threads' maxima has K elements at or above it, and with T >= 2 K threads few more (1.2 to 1.4 K of random data).  After the 2nd, 4th, 8th .. chunk the
 // K-th largest key of the buffer raises it, so that a row of n chunks appends about K (1 + log2 n) keys.  An element that only equals the bar comes
 // behind K others and is left out.  Should the buffer overflow all the same (rising rows), the lanes that found no room wait while it is cut to T keys,
 // and a chunk that alone would fill it is held to the exact K-th of its threads' maxima: K threads, EPT K keys, the room there is.
@@ -448,9 +448,8 @@ template <int T, class Num> __device__ Num top_bound(Num mine, int bits, int K, 
   return b;
 }
 template <int T> struct TopShared { uint64_t all[T]; uint64_t bound; int fill; };
-// the buffer's n keys (0: none) cut to the K largest and at most `most` (K <= most <= T) in all; returns their number and raises the bar
-template <int T, int EPT> __device__ int top_cut(uint64_t* buf, int n, int K, int most, float* bar, TopShared<T>& sh) {
-  constexpr int MOST = EPT / 4 + 1;          // n <= cap = EPT K + T, K <= T / 4
+// the buffer's n <= MOST T keys (0: none) cut to the K largest and at most `most` (K <= most <= T) in all; returns their number and raises the bar
+template <int T, int MOST> __device__ int top_cut(uint64_t* buf, int n, int K, int most, float* bar, TopShared<T>& sh) {
   bool exact = false;
   while (n > most) {
     uint64_t k[MOST], best = 0;
@@ -506,7 +505,7 @@ template <int DT, int T, int U> __device__ __forceinline__ void top_chunk(Pack (
     for (int u = 0; u < U; ++u) if ((ch * U + u) * T + (int)threadIdx.x >= nfull) y[u] = tk_neg<DT>();
   }
 }
-template <int DT, int T, int EPT, int G>
+template <int DT, int T, int EPT, int G, int MOST>
 __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
   constexpr int VEC = Lg<DT>::VEC, U = EPT / VEC;
   extern __shared__ uint64_t buf[];          // [cap]
@@ -610,7 +609,7 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
         for (int q = 1; q < G; ++q) w = q == g ? wait[q] : w;
         const int fill = min(sh.fill, a.cap);
         __syncthreads();
-        top_cut<T, EPT>(buf, fill, K, T, &bar, sh);
+        top_cut<T, MOST>(buf, fill, K, T, &bar, sh);
         over = top_below(top_order(bar));
         uint64_t best = 0;
         for (uint32_t v = w; v; v &= v - 1) {
@@ -636,13 +635,13 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
   __syncthreads();
   int fill = sh.fill;
   __syncthreads();
-  fill = top_cut<T, EPT>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
+  fill = top_cut<T, MOST>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
   if (rem && split == a.nsplit - 1) {        // (cap has room for EPT K more than T)
     if (extra > -INFINITY && extra >= bar) buf[atomicAdd(&sh.fill, 1)] = top_key(extra, ee);   // (those before the vectors count where they equal the bar)
     __syncthreads();
     fill = sh.fill;
     __syncthreads();
-    fill = top_cut<T, EPT>(buf, fill, K, T, &bar, sh);
+    fill = top_cut<T, MOST>(buf, fill, K, T, &bar, sh);
   }
   const MS ms = block_lse<T>(m, s, a.c, red);
   if (a.nsplit > 1) {
@@ -654,7 +653,7 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
   }
 }
 // the splits of a row: their keys are one more buffer to cut
-template <int T, int EPT>
+template <int T, int MOST>
 __global__ __launch_bounds__(T) void top_join_kernel(TopArgs a) {
   extern __shared__ uint64_t buf[];
   __shared__ TopShared<T> sh;
@@ -673,7 +672,7 @@ __global__ __launch_bounds__(T) void top_join_kernel(TopArgs a) {
   float bar = -INFINITY;
   int fill = sh.fill;
   __syncthreads();
-  fill = top_cut<T, EPT>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
+  fill = top_cut<T, MOST>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
   top_write<T>(buf, fill, K, a.idx + r * K, a.val + r * K, nullptr);
 }
 
@@ -706,7 +705,9 @@ TopPlan top_plan(int rows, int V, int K) {
   TopPlan p = {};
   p.nsplit = 1;
   if (V <= 64) return p;                     // top_small_kernel
-  p.threads = K <= 16 && V <= 1024 ? 64 : (K <= 64 ? 256 : (K <= 128 ? 512 : 1024));   // T >= 4 K
+  // T >= 2 K: a chunk's bar leaves 1.4 K of random data above it at most.  T >= 4 K (1.2 K) has fewer blocks on a compute unit: 3840 rows of 100003 fp16,
+  // K = 128, by 512 threads 299 us, by 256 221; 131072 bf16, K = 256, by 1024 558, by 512 372; fp32 and smaller K the same
+  p.threads = K <= 16 && V <= 1024 ? 64 : (K <= 128 ? 256 : 512);
   p.cap = top_ept(p.threads) * K + p.threads;
   const int chunk = p.threads * top_ept(p.threads), nchunk = (V + chunk - 1) / chunk;
   // few rows: split until there are about 512 blocks; the join holds nsplit K <= cap keys
@@ -717,9 +718,10 @@ TopPlan top_plan(int rows, int V, int K) {
   p.ws = p.nsplit > 1 ? (size_t)rows * p.nsplit * ((size_t)K * 8 + sizeof(MS)) : 0;
   return p;
 }
-template <int DT, int T, int EPT, int G> void top_launch(const TopArgs& a, const TopPlan& p, hipStream_t st) {
-  hipLaunchKernelGGL((top_kernel<DT, T, EPT, G>), dim3((uint32_t)a.rows * p.nsplit), dim3(T), p.lds, st, a);
-  if (p.nsplit > 1) hipLaunchKernelGGL((top_join_kernel<T, EPT>), dim3(a.rows), dim3(T), p.lds, st, a);
+template <int DT, int T, int EPT, int G, int KMAX> void top_launch(const TopArgs& a, const TopPlan& p, hipStream_t st) {
+  constexpr int MOST = EPT * KMAX / T + 1;   // cap <= MOST T
+  hipLaunchKernelGGL((top_kernel<DT, T, EPT, G, MOST>), dim3((uint32_t)a.rows * p.nsplit), dim3(T), p.lds, st, a);
+  if (p.nsplit > 1) hipLaunchKernelGGL((top_join_kernel<T, MOST>), dim3(a.rows), dim3(T), p.lds, st, a);
 }
 template <int DT, int G> void top_launch_small(const TopArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((top_small_kernel<DT, G>), dim3((uint32_t)(((int64_t)a.rows * G + 255) / 256)), dim3(256), 0, st, a);
@@ -728,10 +730,10 @@ template <int DT> void top_dispatch(const TopArgs& a, const TopPlan& p, hipStrea
   if (a.V <= 16) top_launch_small<DT, 16>(a, st);
   else if (a.V <= 32) top_launch_small<DT, 32>(a, st);
   else if (a.V <= 64) top_launch_small<DT, 64>(a, st);
-  else if (p.threads == 64) top_launch<DT, 64, 16, 1>(a, p, st);
-  else if (p.threads == 256) top_launch<DT, 256, 32, Lg<DT>::VEC / 4>(a, p, st);
-  else if (p.threads == 512) top_launch<DT, 512, 16, 4>(a, p, st);
-  else top_launch<DT, 1024, 16, 2>(a, p, st);
+  else if (p.threads == 64) top_launch<DT, 64, 16, 1, 16>(a, p, st);
+  else if (p.threads == 256 && a.K <= 64) top_launch<DT, 256, 32, Lg<DT>::VEC / 4, 64>(a, p, st);
+  else if (p.threads == 256) top_launch<DT, 256, 32, Lg<DT>::VEC / 4, 128>(a, p, st);
+  else top_launch<DT, 512, 16, 4, 256>(a, p, st);
 }
 
 // ------------------------------------------------------------------------------------------ drafted tokens against the target

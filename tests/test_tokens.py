@@ -99,7 +99,7 @@ def test_wrappers_check_shapes_and_types():
             with pytest.raises(ValueError, match=text):
                 TK.verify_drafts(here, *args, **kw)
         with pytest.raises(ValueError, match="do not fold"):
-            TK._rows(torch.zeros(3, 4, 10).transpose(0, 1), "logits")
+            TK.top_logits(here, torch.zeros(3, 4, 10).transpose(0, 1), 2)
     finally:
         cpu.undo()
 
