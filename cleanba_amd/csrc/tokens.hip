@@ -255,7 +255,7 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
       for (int k = tid; k < K; k += 64) if (ssame[k]) zm = fmaxf(zm, sz[k]);
       zm = wave_max(zm);
       double zs = 0.0;
-      for (int k = tid; k < K; k += 64) if (ssame[k]) zs += (double)tk_exp2((sz[k] - tk_base(zm)) * a.c);
+      for (int k = tid; k < K; k += 64) if (ssame[k]) zs += exp2(((double)sz[k] - (double)tk_base(zm)) * (double)a.c);
       zs = wave_sum(zs);
       if (tid == 0) stop = MS{zm, zs};
     }
@@ -325,7 +325,9 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   }
   if (S == 0.0 || (!TAIL && sumT == 0.0)) return zeros();   // nothing in the student's row, or nothing in the teacher's (the same for every thread)
   if (tid < 64) {
-    const double logS = log(S), lc = (double)a.c * 0.69314718055994530942;
+    // With a tail, an error of s_T that is in the whole's sum too meets s_T - t_T only; one of the factor that takes it there meets 1: that factor in fp64.
+    const double whole = TAIL ? ms.s * exp2(((double)ms.m - (double)tk_base(M)) * (double)a.c) + stop.s * exp2(((double)stop.m - (double)tk_base(M)) * (double)a.c) : S;
+    const double logS = log(whole), lc = (double)a.c * 0.69314718055994530942;
     double l = 0.0;
     for (int k = tid; k < K; k += 64) if (st[k] != 0.0) l += st[k] * (slt[k] - (((double)sz[k] - (double)M) * lc - logS));
     l = wave_sum(l);
@@ -1257,7 +1259,7 @@ template <int DT> void verify_dispatch(const VerifyArgs& a, const VerifyPlan& p,
 
 // ------------------------------------------------------------------------------------------ entry points: checks, plan, launches
 #define TK_REFUSE(...) do { cbm_set_error(__VA_ARGS__); return -1; } while (0)
-bool tk_temperature(float t) { return t >= 1e-4f && t <= 1e4f; }
+bool tk_temperature(double t) { return t >= 1e-4 && t <= 1e4; }
 int tk_es(int dtype) { return dtype == CBM_F32 ? 4 : 2; }
 int tk_rows(const char* fn, int dtype, int64_t rows, int vocab) {
   if (dtype != CBM_F32 && dtype != CBM_BF16 && dtype != CBM_F16) TK_REFUSE("%s: dtype %d is none of CBM_F32, CBM_BF16, CBM_F16", fn, dtype);
@@ -1302,7 +1304,7 @@ extern "C" int64_t cbm_top_logits_workspace(int32_t dtype, int32_t rows, int32_t
   return rows ? (int64_t)top_plan(rows, vocab, k).ws : 0;
 }
 extern "C" int cbm_top_logits(cbm_ctx* c, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, int32_t k,
-                              float temperature, int32_t* idx, float* values, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+                              double temperature, int32_t* idx, float* values, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* fn = "cbm_top_logits";
   if (tk_rows(fn, dtype, rows, vocab)) return -1;
   if (k < 1 || k > TK_MAX_TOP) TK_REFUSE("%s: k %d outside [1, %d]", fn, k, TK_MAX_TOP);
@@ -1321,7 +1323,7 @@ extern "C" int cbm_top_logits(cbm_ctx* c, const void* logits, int32_t dtype, int
   a.idx = idx; a.val = values; a.lse = lse;
   a.ws_keys = (uint64_t*)workspace; a.ws_ms = (MS*)((char*)workspace + (size_t)rows * p.nsplit * k * 8);
   a.V = vocab; a.K = k; a.rows = rows; a.nsplit = p.nsplit; a.cap = p.cap;
-  a.inv_tau = 1.0 / (double)temperature; a.c = (float)(TK_LOG2E * a.inv_tau);
+  a.inv_tau = 1.0 / temperature; a.c = (float)(TK_LOG2E * a.inv_tau);
   hipStream_t st = tk_stream(c, stream);
   if (dtype == CBM_F32) top_dispatch<CBM_F32>(a, p, st);
   else if (dtype == CBM_BF16) top_dispatch<CBM_BF16>(a, p, st);
@@ -1331,7 +1333,7 @@ extern "C" int cbm_top_logits(cbm_ctx* c, const void* logits, int32_t dtype, int
 
 extern "C" int cbm_distill_loss_grad(cbm_ctx* c, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride,
                                      const int32_t* teacher_idx, const float* teacher_logits, int32_t k, const float* teacher_lse,
-                                     const float* row_weight, float temperature, float* loss, void* dlogits, int64_t grad_stride, void* stream) {
+                                     const float* row_weight, double temperature, float* loss, void* dlogits, int64_t grad_stride, void* stream) {
   const char* fn = "cbm_distill_loss_grad";
   if (tk_rows(fn, dtype, rows, vocab)) return -1;
   if (k < 1 || k > TK_MAX_TOP) TK_REFUSE("%s: k %d outside [1, %d]", fn, k, TK_MAX_TOP);
@@ -1356,7 +1358,7 @@ extern "C" int cbm_distill_loss_grad(cbm_ctx* c, const void* logits, int32_t dty
   a.grad = (char*)dlogits; a.ldg = grad_stride * es;
   a.idx = teacher_idx; a.val = teacher_logits; a.lse = teacher_lse; a.weight = row_weight; a.loss = loss;
   a.rows = rows; a.V = vocab; a.K = k;
-  a.tau = (double)temperature; a.inv_tau = 1.0 / a.tau; a.c = (float)(TK_LOG2E * a.inv_tau);
+  a.tau = temperature; a.inv_tau = 1.0 / a.tau; a.c = (float)(TK_LOG2E * a.inv_tau);
   hipStream_t st = tk_stream(c, stream);
   if (dtype == CBM_F32) distill_dispatch<CBM_F32>(a, st);
   else if (dtype == CBM_BF16) distill_dispatch<CBM_BF16>(a, st);
@@ -1364,25 +1366,25 @@ extern "C" int cbm_distill_loss_grad(cbm_ctx* c, const void* logits, int32_t dty
   return tk_done(fn);
 }
 
-static int verify_check(const char* fn, int dtype, int B, int K, int V, float temperature) {
+static int verify_check(const char* fn, int dtype, int B, int K, int V, double temperature) {
   if (tk_rows(fn, dtype, B, V)) return -1;
   if (K < 0 || K > TK_MAX_DRAFTS) TK_REFUSE("%s: %d drafts outside [0, %d]", fn, K, TK_MAX_DRAFTS);
-  if (!(temperature == 0.0f || tk_temperature(temperature))) TK_REFUSE("%s: temperature %g is neither 0 nor in [1e-4, 1e4]", fn, temperature);
+  if (!(temperature == 0.0 || tk_temperature(temperature))) TK_REFUSE("%s: temperature %g is neither 0 nor in [1e-4, 1e4]", fn, temperature);
   if ((int64_t)B * (2 * K + 1) > (1 << 24)) TK_REFUSE("%s: %d sequences of %d drafts are more than 2^24 rows", fn, B, K);
   return 0;
 }
-extern "C" int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, float temperature) {
+extern "C" int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, double temperature) {
   if (verify_check("cbm_verify_drafts_workspace", dtype, batch, drafts, vocab, temperature)) return -1;
-  return batch ? (int64_t)verify_plan(batch, drafts, vocab, with_draft_logits != 0, temperature == 0.0f).ws : 0;
+  return batch ? (int64_t)verify_plan(batch, drafts, vocab, with_draft_logits != 0, temperature == 0.0).ws : 0;
 }
 extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab,
                                  int64_t target_batch_stride, int64_t target_pos_stride, const void* draft_logits, int64_t draft_batch_stride,
                                  int64_t draft_pos_stride, const int32_t* draft_tokens, const int32_t* n_draft, const float* u_accept,
-                                 const float* u_sample, float temperature, int32_t* tokens, int32_t* accepted, float* logprobs, void* workspace,
+                                 const float* u_sample, double temperature, int32_t* tokens, int32_t* accepted, float* logprobs, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   const char* fn = "cbm_verify_drafts";
   if (verify_check(fn, dtype, batch, drafts, vocab, temperature)) return -1;
-  const bool greedy = temperature == 0.0f;
+  const bool greedy = temperature == 0.0;
   if ((drafts > 0 && target_pos_stride < 0) || (batch > 1 && target_batch_stride < 0)) TK_REFUSE("%s: negative stride", fn);
   if (draft_logits && ((drafts > 1 && draft_pos_stride < 0) || (batch > 1 && draft_batch_stride < 0))) TK_REFUSE("%s: negative stride", fn);
   if (batch == 0) { if (!c) TK_REFUSE("%s: null context", fn); return 0; }
@@ -1406,7 +1408,7 @@ extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t 
   char* ws = (char*)workspace;
   a.sums = (VfSum*)ws; a.parts = (VfSum*)(ws + p.o_parts); a.rest = (double*)(ws + p.o_rest); a.stats = (MS*)(ws + p.o_stats); a.done = (uint32_t*)(ws + p.o_done);
   a.B = batch; a.K = drafts; a.V = vocab; a.nsplit = p.nsplit; a.nchunk = p.nchunk; a.nstat = p.nstat; a.npick = p.npick;
-  a.C = greedy ? 0.0 : TK_LOG2E / (double)temperature; a.c = (float)a.C;
+  a.C = greedy ? 0.0 : TK_LOG2E / temperature; a.c = (float)a.C;
   hipStream_t st = tk_stream(c, stream);
   if (dtype == CBM_F32) verify_dispatch<CBM_F32>(a, p, greedy, st);
   else if (dtype == CBM_BF16) verify_dispatch<CBM_BF16>(a, p, greedy, st);

@@ -131,14 +131,14 @@ def load():
     lib.cbm_synth_env_step_host_to.argtypes = [C.c_uint32, C.c_int32, C.c_int32, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.cbm_comm_load.argtypes = [C.c_char_p]
     lib.cbm_comm_backend.restype = C.c_char_p
-    i32, i64, f32 = C.c_int32, C.c_int64, C.c_float
+    i32, i64, f64 = C.c_int32, C.c_int64, C.c_double
     lib.cbm_top_logits_workspace.restype = i64
     lib.cbm_top_logits_workspace.argtypes = [i32, i32, i32, i32]
-    lib.cbm_top_logits.argtypes = [vp, vp, i32, i32, i32, i64, i32, f32, vp, vp, vp, vp, i64, vp]
-    lib.cbm_distill_loss_grad.argtypes = [vp, vp, i32, i32, i32, i64, vp, vp, i32, vp, vp, f32, vp, vp, i64, vp]
+    lib.cbm_top_logits.argtypes = [vp, vp, i32, i32, i32, i64, i32, f64, vp, vp, vp, vp, i64, vp]
+    lib.cbm_distill_loss_grad.argtypes = [vp, vp, i32, i32, i32, i64, vp, vp, i32, vp, vp, f64, vp, vp, i64, vp]
     lib.cbm_verify_drafts_workspace.restype = i64
-    lib.cbm_verify_drafts_workspace.argtypes = [i32, i32, i32, i32, i32, f32]
-    lib.cbm_verify_drafts.argtypes = [vp, vp, i32, i32, i32, i32, i64, i64, vp, i64, i64, vp, vp, vp, vp, f32, vp, vp, vp, vp, i64, vp]
+    lib.cbm_verify_drafts_workspace.argtypes = [i32, i32, i32, i32, i32, f64]
+    lib.cbm_verify_drafts.argtypes = [vp, vp, i32, i32, i32, i32, i64, i64, vp, i64, i64, vp, vp, vp, vp, f64, vp, vp, vp, vp, i64, vp]
     _lib = lib
     return lib
 

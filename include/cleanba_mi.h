@@ -299,7 +299,7 @@ enum { CBM_F32 = 0, CBM_BF16 = 1, CBM_F16 = 2 };
  * lse f32 [rows] = log sum_j exp(logits_j / tau).  -inf and NaN are never taken; a slot that stays empty holds idx -1, value -inf.  A row of nothing
  * but -inf has lse -inf, one with a NaN lse NaN, one with +inf lse +inf. */
 int64_t cbm_top_logits_workspace(int32_t dtype, int32_t rows, int32_t vocab, int32_t k);
-int cbm_top_logits(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, int32_t k, float temperature,
+int cbm_top_logits(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, int32_t k, double temperature,
                    int32_t* idx, float* values, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 /* Distillation from a teacher's top logits: KL(teacher || student) tau^2 per row times row_weight (NULL: 1), and its gradient.
  *  teacher_idx i32 [rows][k], teacher_logits f32 [rows][k] (k 1..256): the teacher's slots; an index outside [0, vocab) is an empty slot, a token in
@@ -310,7 +310,7 @@ int cbm_top_logits(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows
  * Loss and gradient of a row are 0 where its weight is 0 (the row is not read), where all its logits are -inf, and where the teacher has no filled slot.
  * The class of other tokens is left out where the student has no logit above -inf for it.  A student's -inf on a token of the teacher gives loss +inf. */
 int cbm_distill_loss_grad(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, const int32_t* teacher_idx,
-                          const float* teacher_logits, int32_t k, const float* teacher_lse, const float* row_weight, float temperature, float* loss,
+                          const float* teacher_logits, int32_t k, const float* teacher_lse, const float* row_weight, double temperature, float* loss,
                           void* dlogits, int64_t grad_stride, void* stream);
 /* Verification of drafted tokens against the target's distributions p, from given random numbers; keeps the target's distribution exactly.
  *  target_logits [batch][drafts+1][vocab], draft_logits [batch][drafts][vocab] or NULL (drafts that were looked up: q is one-hot at the token), strides in
@@ -323,10 +323,10 @@ int cbm_distill_loss_grad(cbm_ctx* ctx, const void* logits, int32_t dtype, int32
  *    looked at and may be NULL, logprobs are 0.
  *  A token outside [0, vocab) is rejected; so is one whose draft row is no distribution (only -inf, a NaN or +inf), and then the token is drawn from p.
  *  A target row that is no distribution rejects, and the drawn token is -1.  drafts = 0 samples one token a sequence. */
-int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, float temperature);
+int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, double temperature);
 int cbm_verify_drafts(cbm_ctx* ctx, const void* target_logits, int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int64_t target_batch_stride,
                       int64_t target_pos_stride, const void* draft_logits, int64_t draft_batch_stride, int64_t draft_pos_stride,
-                      const int32_t* draft_tokens, const int32_t* n_draft, const float* u_accept, const float* u_sample, float temperature,
+                      const int32_t* draft_tokens, const int32_t* n_draft, const float* u_accept, const float* u_sample, double temperature,
                       int32_t* tokens, int32_t* accepted, float* logprobs, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- per-kernel HIP-event timing for bench.py's roofline line: brackets every learner-stream launch of
