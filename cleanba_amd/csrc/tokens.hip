@@ -385,10 +385,10 @@ void distill_launch(const DistillArgs& a, hipStream_t st) {
   if (a.lse) hipLaunchKernelGGL((distill_kernel<DT, T, NV, true>), dim3(a.rows), dim3(T), ((a.V + 31) / 32 + 1) * 4, st, a);
   else hipLaunchKernelGGL((distill_kernel<DT, T, NV, false>), dim3(a.rows), dim3(T), 0, st, a);
 }
-// 8 vectors a thread stay; a block of 256, 512 or 1024 threads has 6, 3 or 1.5 others beside it on its compute unit, whose loads, sums and stores overlap its
-// own.  A larger block reads less of its row twice, a smaller one has more company.  3840 rows with gradient, us by blocks of 256 / 512 / 1024:
+// 8 vectors a thread stay (80 registers); 6 blocks of 256 threads share a compute unit, 3 of 512, and one of 1024 is alone there: the loads, sums and stores of
+// neighbours overlap.  A larger block reads less of its row twice, a smaller one has more company.  3840 rows with gradient, us by blocks of 256 / 512 / 1024:
 // 20000 bf16 (2500 vectors) 70 / 86 / 144, 32768 bf16 122 / 106 / 170, 65536 bf16 (8192) 260 / 216 / 251, 50021 fp32 (12506) 453 / 358 / 325,
-// 131072 bf16 (16384) 575 / 470 / 427.  16 vectors a thread: 431 there, 200 against 140 at 40000 bf16 (two blocks of 150 registers do not fit).  K <= T.
+// 131072 bf16 (16384) 575 / 470 / 427.  12 or 16 vectors a thread: 424 and 442 there, 320 and 318 at 50021 fp32.  K <= T.
 template <int DT>
 void distill_dispatch(const DistillArgs& a, hipStream_t st) {
   const int nv = (a.V + Lg<DT>::VEC - 1) / Lg<DT>::VEC;
@@ -452,8 +452,8 @@ template <int T, class Num> __device__ Num top_bound(Num mine, int bits, int K, 
 template <int T> struct TopShared { uint64_t all[T]; uint64_t bound; int fill; };
 // the buffer's n <= MOST T keys (0: none) cut to the K largest and at most `most` (K <= most <= T) in all; returns their number and raises the bar
 template <int T, int MOST> __device__ int top_cut(uint64_t* buf, int n, int K, int most, float* bar, TopShared<T>& sh) {
-  bool exact = false;
-  while (n > most) {
+  // Of n > T keys, ceil(n / T) a thread, an exact cut leaves ceil(n / T) K, as T >= 2 K at most half and a bit: 8 turns are more than it takes.
+  for (int turn = 0; n > most && turn < 8; ++turn) {
     uint64_t k[MOST], best = 0;
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
@@ -461,7 +461,7 @@ template <int T, int MOST> __device__ int top_cut(uint64_t* buf, int n, int K, i
       best = k[i] > best ? k[i] : best;
     }
     uint64_t bound;                          // (its barriers stand between the reads above and the writes below)
-    if (exact) bound = top_bound<T, uint64_t>(best, TOP_KEY_BITS, K, 0, sh.all, &sh.bound);
+    if (turn > 0) bound = top_bound<T, uint64_t>(best, TOP_KEY_BITS, K, 0, sh.all, &sh.bound);   // (equal values may have kept too many: now their indices tell them apart)
     else bound = (uint64_t)top_bound<T, uint32_t>(top_order_of(best), 32, K, K / 4, (uint32_t*)sh.all, (uint32_t*)&sh.bound) << 19;
     if (bound) *bar = fmaxf(*bar, top_value(top_order_of(bound)));
     if (threadIdx.x == 0) sh.fill = 0;
@@ -470,14 +470,13 @@ template <int T, int MOST> __device__ int top_cut(uint64_t* buf, int n, int K, i
     for (int i = 0; i < MOST; ++i) if (k[i] != 0 && k[i] >= bound) buf[atomicAdd(&sh.fill, 1)] = k[i];
     __syncthreads();
     n = sh.fill;
-    exact = true;                            // (equal values may have kept too many: the next turn tells them apart by their indices)
     __syncthreads();
   }
   return n;
 }
 // writes the buffer's K largest in order; n <= T
 template <int T> __device__ void top_write(const uint64_t* buf, int n, int K, int32_t* idx, float* val, uint64_t* keys) {
-  if ((int)threadIdx.x < n) {
+  if ((int)threadIdx.x < n) {                // (n <= T)
     const uint64_t mine = buf[threadIdx.x];
     int rank = 0;
 #pragma unroll 4
@@ -539,6 +538,8 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        vm[g][u] = -INFINITY;
+        if (((c + g) * U + u) * T >= nfull) continue;   // (the same for every thread: short rows do not fill a group)
         vm[g][u] = tk_max<DT>(x[g][u]);
         cm = fmaxf(cm, vm[g][u]);
         tk_redecode(x[g][u]);
@@ -549,7 +550,11 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int u = 0; u < U; ++u) { p += es.sum<DT>(x[g][u]); tk_redecode(x[g][u]); }
+      for (int u = 0; u < U; ++u) {
+        if (((c + g) * U + u) * T >= nfull) continue;
+        p += es.sum<DT>(x[g][u]);
+        tk_redecode(x[g][u]);
+      }
     p *= es.fix;
     if (es.far) {
       p = 0.0f;
@@ -702,16 +707,16 @@ __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a) {
 }
 
 struct TopPlan { int threads, nsplit, cap; size_t lds, ws; };
-int top_ept(int threads) { return threads == 256 ? 32 : 16; }
+int top_ept(int threads, int V) { return threads == 256 ? 32 : (threads == 512 && V <= 4096 ? 8 : 16); }
 TopPlan top_plan(int rows, int V, int K) {
   TopPlan p = {};
   p.nsplit = 1;
   if (V <= 64) return p;                     // top_small_kernel
   // T >= 2 K: a chunk's bar leaves 1.4 K of random data above it at most.  T >= 4 K (1.2 K) has fewer blocks on a compute unit: 3840 rows of 100003 fp16,
   // K = 128, by 512 threads 299 us, by 256 221; 131072 bf16, K = 256, by 1024 558, by 512 372; fp32 and smaller K the same
-  p.threads = K <= 16 && V <= 1024 ? 64 : (K <= 128 ? 256 : 512);
-  p.cap = top_ept(p.threads) * K + p.threads;
-  const int chunk = p.threads * top_ept(p.threads), nchunk = (V + chunk - 1) / chunk;
+  p.threads = K <= 32 && V <= 1024 ? 64 : (K <= 64 && V <= 2048 ? 128 : (K <= 128 ? 256 : 512));
+  p.cap = top_ept(p.threads, V) * K + p.threads;
+  const int chunk = p.threads * top_ept(p.threads, V), nchunk = (V + chunk - 1) / chunk;
   // few rows: split until there are about 512 blocks; the join holds nsplit K <= cap keys
   int n = rows >= 512 ? 1 : (512 + rows - 1) / rows;
   n = n < nchunk ? n : nchunk;
@@ -721,6 +726,7 @@ TopPlan top_plan(int rows, int V, int K) {
   return p;
 }
 template <int DT, int T, int EPT, int G, int KMAX> void top_launch(const TopArgs& a, const TopPlan& p, hipStream_t st) {
+  static_assert(2 * KMAX <= T, "or top_cut does not end");
   constexpr int MOST = EPT * KMAX / T + 1;   // cap <= MOST T
   hipLaunchKernelGGL((top_kernel<DT, T, EPT, G, MOST>), dim3((uint32_t)a.rows * p.nsplit), dim3(T), p.lds, st, a);
   if (p.nsplit > 1) hipLaunchKernelGGL((top_join_kernel<T, MOST>), dim3(a.rows), dim3(T), p.lds, st, a);
@@ -732,9 +738,11 @@ template <int DT> void top_dispatch(const TopArgs& a, const TopPlan& p, hipStrea
   if (a.V <= 16) top_launch_small<DT, 16>(a, st);
   else if (a.V <= 32) top_launch_small<DT, 32>(a, st);
   else if (a.V <= 64) top_launch_small<DT, 64>(a, st);
-  else if (p.threads == 64) top_launch<DT, 64, 16, 1, 16>(a, p, st);
+  else if (p.threads == 64) top_launch<DT, 64, 16, 1, 32>(a, p, st);
+  else if (p.threads == 128) top_launch<DT, 128, 16, 1, 64>(a, p, st);
   else if (p.threads == 256 && a.K <= 64) top_launch<DT, 256, 32, Lg<DT>::VEC / 4, 64>(a, p, st);
   else if (p.threads == 256) top_launch<DT, 256, 32, Lg<DT>::VEC / 4, 128>(a, p, st);
+  else if (a.V <= 4096) top_launch<DT, 512, 8, 1, 256>(a, p, st);
   else top_launch<DT, 512, 16, 4, 256>(a, p, st);
 }
 
