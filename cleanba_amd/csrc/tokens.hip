@@ -476,8 +476,9 @@ template <int T, int MOST> __device__ int top_cut(uint64_t* buf, int n, int K, i
 }
 // writes the buffer's K largest in order; n <= T
 template <int T> __device__ void top_write(const uint64_t* buf, int n, int K, int32_t* idx, float* val, uint64_t* keys) {
-  if ((int)threadIdx.x < n) {                // (n <= T)
-    const uint64_t mine = buf[threadIdx.x];
+  const uint64_t mine = (int)threadIdx.x < n ? buf[threadIdx.x] : 0;   // (n <= T; a 0 is no key)
+  const int live = __syncthreads_count(mine != 0);
+  if (mine) {
     int rank = 0;
 #pragma unroll 4
     for (int j = 0; j < n; ++j) rank += buf[j] > mine;
@@ -486,7 +487,7 @@ template <int T> __device__ void top_write(const uint64_t* buf, int n, int K, in
       else { idx[rank] = top_index(mine); val[rank] = top_value(top_order_of(mine)); }
     }
   }
-  for (int k = n + (int)threadIdx.x; k < K; k += T) {
+  for (int k = live + (int)threadIdx.x; k < K; k += T) {
     if (keys) keys[k] = 0;
     else { idx[k] = -1; val[k] = -INFINITY; }
   }
@@ -666,9 +667,7 @@ __global__ __launch_bounds__(T) void top_join_kernel(TopArgs a) {
   __shared__ TopShared<T> sh;
   const int tid = threadIdx.x, K = a.K, n = a.nsplit * K;
   const int64_t r = blockIdx.x;
-  if (tid == 0) sh.fill = 0;
-  __syncthreads();
-  for (int i = tid; i < n; i += T) { const uint64_t k = a.ws_keys[r * n + i]; if (k) buf[atomicAdd(&sh.fill, 1)] = k; }
+  for (int i = tid; i < n; i += T) buf[i] = a.ws_keys[r * n + i];
   if (tid < 64) {
     MS ms = tid < a.nsplit ? a.ws_ms[r * a.nsplit + tid] : MS{-INFINITY, 0.0};
     const float M = wave_max(ms.m);
@@ -677,9 +676,7 @@ __global__ __launch_bounds__(T) void top_join_kernel(TopArgs a) {
   }
   __syncthreads();
   float bar = -INFINITY;
-  int fill = sh.fill;
-  __syncthreads();
-  fill = top_cut<T, MOST>(buf, fill, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
+  int fill = top_cut<T, MOST>(buf, n, K, 3 * K + 32 < T ? 3 * K + 32 : T, &bar, sh);
   top_write<T>(buf, fill, K, a.idx + r * K, a.val + r * K, nullptr);
 }
 
@@ -715,12 +712,17 @@ TopPlan top_plan(int rows, int V, int K) {
   // T >= 2 K: a chunk's bar leaves 1.4 K of random data above it at most.  T >= 4 K (1.2 K) has fewer blocks on a compute unit: 3840 rows of 100003 fp16,
   // K = 128, by 512 threads 299 us, by 256 221; 131072 bf16, K = 256, by 1024 558, by 512 372; fp32 and smaller K the same
   p.threads = K <= 32 && V <= 1024 ? 64 : (K <= 64 && V <= 2048 ? 128 : (K <= 128 ? 256 : 512));
+  // Few rows leave compute units empty: up to 128 long ones are split until there are about 512 blocks, and joined (a second kernel); up to 255 others go to
+  // wider blocks.  us split / not: 60 x 32768 bf16, K = 32, 20 / 15; 1 x 131072 bf16, K = 64, 21 / 30; 60 of them 21 / 31, 200 34 / 34; 1 x 100003 fp16, K = 128, 27 / 31,
+  // 200 39 / 36; K = 256 (by 512 threads either way) 1 x 131072 38 / 40, 60 58 / 40.
+  const bool split = rows <= 128 && V > 49152 && K <= 128;
+  if (!split && rows < 256 && V > 16384) p.threads = 512;
   p.cap = top_ept(p.threads, V) * K + p.threads;
-  const int chunk = p.threads * top_ept(p.threads, V), nchunk = (V + chunk - 1) / chunk;
-  // few rows: split until there are about 512 blocks; the join holds nsplit K <= cap keys
-  int n = rows >= 512 ? 1 : (512 + rows - 1) / rows;
-  n = n < nchunk ? n : nchunk;
-  p.nsplit = n < 16 ? n : 16;
+  if (split) {
+    const int chunk = p.threads * top_ept(p.threads, V), nchunk = (V + chunk - 1) / chunk, n = (512 + rows - 1) / rows;
+    p.nsplit = n < nchunk ? n : nchunk;
+    p.nsplit = p.nsplit < 16 ? p.nsplit : 16;   // (the join holds nsplit K <= cap keys)
+  }
   p.lds = (size_t)p.cap * 8;
   p.ws = p.nsplit > 1 ? (size_t)rows * p.nsplit * ((size_t)K * 8 + sizeof(MS)) : 0;
   return p;
