@@ -14,6 +14,7 @@ namespace {
 constexpr int TK_MAX_VOCAB = 1 << 19;   // indices are 19 bits of a key in the top-K kernels; a row's bitmap (one bit a token) fits 64 KB of LDS
 constexpr int TK_MAX_TOP = 256;         // slots of a row: four a lane of the wave that owns the row's teacher
 constexpr int TK_MAX_DRAFTS = 128;      // one thread a draft in the acceptance step
+constexpr int TK_MAX_ROWS = 1 << 22;    // a launch holds fewer than 2^32 threads, a row up to 1024
 
 // ------------------------------------------------------------------------------------------ 16 bytes of logits
 typedef uint32_t tk_u4 __attribute__((ext_vector_type(4)));
@@ -779,7 +780,7 @@ struct VerifyArgs {
   uint32_t* done;                            // [sequence]: blocks that have finished; cleared by the first kernel for the second
   int B, K, V, nchunk, nstat, nsplit, npick; // splits of a row in fp32 and in fp64, blocks a sequence in the last kernel
   float c;
-  double C;
+  double C, C2;                              // log2(e) / tau, and the power of two not below it
 };
 __device__ __forceinline__ int vf_drafts(const VerifyArgs& a, int b) {
   const int n = a.n_draft ? a.n_draft[b] : a.K;
@@ -805,9 +806,19 @@ struct VfExp {
     return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)((n & ~31u) << 15) << 32));   // k into the exponent
   }
 };
+// The whole number E of a maximum m: m C rounded up.  Beyond 2^36 a float's neighbours differ by 2^12 and more in the exponent, so that beside m all but its
+// equals are nothing, but m C itself is rounded by more and more: there C is replaced by the power of two above it, which makes m C2 exact, and whole.
+// vf_slope says from E which of the two it was made with.
+constexpr double VF_FAR = 0x1p36;
+__device__ __forceinline__ double vf_slope(const VerifyArgs& a, double e) { return fabs(e) > VF_FAR ? a.C2 : a.C; }
+__device__ __forceinline__ double vf_ceil(const VerifyArgs& a, float m) {
+  if (m == -INFINITY) return 0.0;
+  const double e = ceil((double)m * a.C);
+  return fabs(e) > VF_FAR ? (double)m * a.C2 : e;
+}
 // probability of logit z in a row of sum `s`; what VF_NOTHING stands for is 0
-__device__ __forceinline__ double vf_prob(const double* table, double C, const VfSum& s, float z) {
-  const double e = VfExp{table, 32.0 * C, 32.0 * s.e}(z);
+__device__ __forceinline__ double vf_prob(const double* table, const VerifyArgs& a, const VfSum& s, float z) {
+  const double e = VfExp{table, 32.0 * vf_slope(a, s.e), 32.0 * s.e}(z);
   return e > 2.0 * VF_NOTHING ? e / s.s : 0.0;
 }
 __device__ __forceinline__ double vf_scaled(const VfSum& x, double e) { return x.e == e ? x.s : ldexp(x.s, (int)fmax(x.e - e, -4000.0)); }   // s 2^(x.e - e)
@@ -816,7 +827,9 @@ __device__ __forceinline__ VfSum vf_add(const VfSum& x, const VfSum& y) {
   return VfSum{e, vf_scaled(x, e) + vf_scaled(y, e)};
 }
 __device__ __forceinline__ bool vf_good(const VfSum& x) { return x.e > -INFINITY && x.e < INFINITY && x.s > 0.0; }
-__device__ __forceinline__ double vf_ceil(float m, double C) { return m == -INFINITY ? 0.0 : ceil((double)m * C); }
+__device__ __forceinline__ double vf_logp(const VerifyArgs& a, const VfSum& s, float z) {
+  return ((double)z * vf_slope(a, s.e) - s.e) * 0.69314718055994530942 - log(s.s);
+}
 
 // (maximum, sum) of a share of one drafted position's row
 template <int DT>
@@ -891,7 +904,8 @@ template <int DT, bool ALL> __device__ int vf_accept(const VerifyArgs& a, int b,
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
       for (int i = tid & 15; i < a.nstat; i += 16) s.s += p[i].s * (double)tk_exp2((p[i].m - tk_base(m)) * a.c);
       for (int o = 8; o > 0; o >>= 1) s.s += __shfl_xor(s.s, o, 16);
-      s.e = (double)m * a.C;
+      s.e = m == -INFINITY ? m : vf_ceil(a, m);
+      if ((tid & 15) == 0) s.s *= exp2(fma((double)m, vf_slope(a, s.e), -s.e));   // (the sum was relative to m)
     }
     if ((tid & 15) == 0) srow[r] = s;
   }
@@ -901,14 +915,14 @@ template <int DT, bool ALL> __device__ int vf_accept(const VerifyArgs& a, int b,
     bool ok = false;
     if ((uint32_t)x < (uint32_t)a.V && vf_good(srow[tid])) {
       const VfSum ps = srow[tid];
-      const double p = vf_prob(table, a.C, ps, zp);
+      const double p = vf_prob(table, a, ps, zp);
       double q = 1.0;
       if (a.draft) {
         const VfSum qs = srow[heads + tid];
-        q = vf_good(qs) ? vf_prob(table, a.C, qs, zq) : NAN;
+        q = vf_good(qs) ? vf_prob(table, a, qs, zq) : NAN;
       }
       ok = (double)u * q < p;                // (a NaN: not accepted)
-      if (ok && write) logp = ((double)zp * a.C - ps.e) * 0.69314718055994530942 - log(ps.s);
+      if (ok && write) logp = vf_logp(a, ps, zp);
     }
     if (!ok) atomicMin(sat, tid);
   }
@@ -986,8 +1000,8 @@ __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
       for (int j = 0; j < VEC; j += 2) nan |= __ballot(__builtin_isunordered(tk_get<DT>(x[u], j), tk_get<DT>(x[u], j + 1)));
     }
     m = wave_max(m);
-    const double E = vf_ceil(m, a.C);
-    const VfExp ex = {table, 32.0 * a.C, 32.0 * E};
+    const double E = vf_ceil(a, m);
+    const VfExp ex = {table, 32.0 * vf_slope(a, E), 32.0 * E};
     double s = 0.0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1065,7 +1079,7 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
   const char* prow = a.target + b * a.tb + at * a.tp;
   const char* qrow = a.draft && at < n && vf_good(srow[qrow_at]) ? a.draft + b * a.db + at * a.dp : nullptr;
   const VfSum qs = qrow ? srow[qrow_at] : VfSum{0.0, 1.0};
-  const VfExp ep = {table, 32.0 * a.C, 32.0 * ps.e}, eq = {table, 32.0 * a.C, 32.0 * qs.e};
+  const VfExp ep = {table, 32.0 * vf_slope(a, ps.e), 32.0 * ps.e}, eq = {table, 32.0 * vf_slope(a, qs.e), 32.0 * qs.e};
   const double np = 1.0 / ps.s, nq = 1.0 / qs.s, none = 2.0 * VF_NOTHING * np;
   bool rest = qrow != nullptr;
   if (rest) {
@@ -1114,7 +1128,9 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
     const auto chunk = [&](int i) {
       if (i >= a.nchunk) return 0.0;
       if (rest) return (double)__hip_atomic_load(&a.rest[(int64_t)b * a.nchunk + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      return skip >= 0 && i == skip / VF_CHUNK ? without : vf_scaled(sums[i], ps.e) * np;
+      if (skip >= 0 && i == skip / VF_CHUNK) return without;
+      // a chunk that counts has a token that counts: its largest is above 2^-991 of the row's, and weight() leaves out what is below 2^-999
+      return sums[i].e - ps.e >= -990.0 ? vf_scaled(sums[i], ps.e) * np : 0.0;
     };
     double mine = 0.0;
     for (int j = 0; j < per; ++j) mine += chunk(tid * per + j);
@@ -1159,7 +1175,7 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
   if (tid == 0) {
     const int token = sfirst < a.V ? sfirst : slast;
     a.out[o] = token;
-    if (a.logprobs) a.logprobs[o] = (float)(((double)tk_at<DT>(prow, token) * a.C - ps.e) * 0.69314718055994530942 - log(ps.s));
+    if (a.logprobs) a.logprobs[o] = (float)vf_logp(a, ps, tk_at<DT>(prow, token));
   }
 }
 
@@ -1274,7 +1290,7 @@ int tk_es(int dtype) { return dtype == CBM_F32 ? 4 : 2; }
 int tk_rows(const char* fn, int dtype, int64_t rows, int vocab) {
   if (dtype != CBM_F32 && dtype != CBM_BF16 && dtype != CBM_F16) TK_REFUSE("%s: dtype %d is none of CBM_F32, CBM_BF16, CBM_F16", fn, dtype);
   if (vocab < 1 || vocab > TK_MAX_VOCAB) TK_REFUSE("%s: vocab %d outside [1, %d]", fn, vocab, TK_MAX_VOCAB);
-  if (rows < 0 || rows > (1 << 24)) TK_REFUSE("%s: %lld rows outside [0, 2^24]", fn, (long long)rows);
+  if (rows < 0 || rows >= TK_MAX_ROWS) TK_REFUSE("%s: %lld rows outside [0, 2^22)", fn, (long long)rows);
   return 0;
 }
 int tk_pointer(const char* fn, const char* name, const void* p, size_t align) {
@@ -1380,7 +1396,7 @@ static int verify_check(const char* fn, int dtype, int B, int K, int V, double t
   if (tk_rows(fn, dtype, B, V)) return -1;
   if (K < 0 || K > TK_MAX_DRAFTS) TK_REFUSE("%s: %d drafts outside [0, %d]", fn, K, TK_MAX_DRAFTS);
   if (!(temperature == 0.0 || tk_temperature(temperature))) TK_REFUSE("%s: temperature %g is neither 0 nor in [1e-4, 1e4]", fn, temperature);
-  if ((int64_t)B * (2 * K + 1) > (1 << 24)) TK_REFUSE("%s: %d sequences of %d drafts are more than 2^24 rows", fn, B, K);
+  if ((int64_t)B * (2 * K + 1) >= TK_MAX_ROWS) TK_REFUSE("%s: %d sequences of %d drafts are 2^22 rows or more", fn, B, K);
   return 0;
 }
 extern "C" int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, double temperature) {
@@ -1418,7 +1434,7 @@ extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t 
   char* ws = (char*)workspace;
   a.sums = (VfSum*)ws; a.parts = (VfSum*)(ws + p.o_parts); a.rest = (double*)(ws + p.o_rest); a.stats = (MS*)(ws + p.o_stats); a.done = (uint32_t*)(ws + p.o_done);
   a.B = batch; a.K = drafts; a.V = vocab; a.nsplit = p.nsplit; a.nchunk = p.nchunk; a.nstat = p.nstat; a.npick = p.npick;
-  a.C = greedy ? 0.0 : TK_LOG2E / temperature; a.c = (float)a.C;
+  a.C = greedy ? 0.0 : TK_LOG2E / temperature; a.C2 = greedy ? 0.0 : std::exp2(std::ceil(std::log2(a.C))); a.c = (float)a.C;
   hipStream_t st = tk_stream(c, stream);
   if (dtype == CBM_F32) verify_dispatch<CBM_F32>(a, p, greedy, st);
   else if (dtype == CBM_BF16) verify_dispatch<CBM_BF16>(a, p, greedy, st);

@@ -292,6 +292,7 @@ int cbm_rmsprop_step(cbm_ctx* ctx, float* p, const float* g, float* nu, int64_t 
  *    streams may call at once and calls may be captured into graphs.  The caller's current device is left as it was.
  *  - The workspace is the caller's: at least cbm_*_workspace(...) bytes (0: may be NULL) at 16-byte alignment, contents irrelevant, not shared by calls
  *    that may run at the same time.  The *_workspace functions return -1 for sizes that the operator refuses.
+ *  - Fewer than 2^22 rows a call (cbm_verify_drafts: batch (2 drafts + 1)).  No output overlaps another array, but for the gradient written in place.
  *  - temperature tau in [1e-4, 1e4]: distributions are softmax(logits / tau). */
 enum { CBM_F32 = 0, CBM_BF16 = 1, CBM_F16 = 2 };
 #define CBM_LEARNER_STREAM ((void*)(intptr_t)-1)
@@ -314,8 +315,8 @@ int cbm_distill_loss_grad(cbm_ctx* ctx, const void* logits, int32_t dtype, int32
                           void* dlogits, int64_t grad_stride, void* stream);
 /* Verification of drafted tokens against the target's distributions p, from given random numbers; keeps the target's distribution exactly.
  *  target_logits [batch][drafts+1][vocab], draft_logits [batch][drafts][vocab] or NULL (drafts that were looked up: q is one-hot at the token), strides in
- *    elements (0 allowed: shared rows); draft_tokens i32 [batch][drafts]; n_draft i32 [batch] or NULL: how many of them count (clamped to [0, drafts]; rows behind are not read);
- *    u_accept f32 [batch][drafts], u_sample f32 [batch] in [0, 1).
+ *    elements (0 allowed: shared rows); draft_tokens i32 [batch][drafts]; n_draft i32 [batch] or NULL: how many of them count (clamped to [0, drafts];
+ *    rows behind are not read); u_accept f32 [batch][drafts], u_sample f32 [batch] in [0, 1).
  *  Draft i is accepted while u_accept_i q_i(x_i) < p_i(x_i).  At the first rejection a one token is drawn from max(p_a - q_a, 0) (from p_a where that is 0
  *    everywhere), after n acceptances from p_n: the first token whose cumulative weight exceeds u_sample times the whole.
  *  tokens i32 [batch][drafts+1]: the accepted ones, the drawn one, then -1; accepted i32 [batch]; logprobs f32 [batch][drafts+1] or NULL: log p of each

@@ -418,6 +418,55 @@ def test_verify_extreme_random_numbers(ctx):
     assert np.allclose(lp.cpu().numpy(), -math.log(live.size), atol=D(V) + 1e-6)
 
 
+@pytest.mark.parametrize("V, times", [(30, 1), (9000, 1), (30, 40000), (9000, 120)])
+def test_verify_huge_logits(ctx, V, times):
+    """Rows whose largest logit is a mask's lowest value, two such levels, the largest floats: equal ones share, all others have nothing.  Once, and as a large call."""
+    rng = np.random.default_rng(V)
+    low = -float(torch.finfo(torch.float32).max)
+    B, K = 6, 2
+    p = rng.normal(0, 3, (B, K + 1, V)).astype(np.float32)
+    q = rng.normal(0, 3, (B, K, V)).astype(np.float32)
+    q[:] = p[:, :K] + rng.normal(0, 0.3, q.shape)
+    x = rng.integers(0, V, (B, K)).astype(np.int32)
+    ua, us = rng.random((B, K), dtype=np.float32) * np.float32(0.5), rng.random(B, dtype=np.float32)
+    p[0] = low                                # uniform
+    q[0] = low
+    p[1] = low                                # a level above the lowest: it alone
+    p[1, :, 5:15] = -1e30
+    x[1] = 5, 20
+    q[1] = p[1, :K]
+    p[2] = 1e38                               # the neighbour below the largest
+    p[2, :, 3:7] = np.nextafter(np.float32(1e38), np.float32(np.inf))
+    x[2] = 4, 2
+    p[3] = np.where(rng.random((K + 1, V)) < 0.9, low, p[3]).astype(np.float32)   # an ordinary masked row
+    q[3] = low                                # drafted from a uniform row
+    x[3] = p[3, :K].argmax(1)
+    p[4] = np.where(np.arange(V) % 2, np.float32(2.0**37), -np.float32(2.0**37))
+    x[4] = 1, 2
+    p[5] = 7e10 + 8192 * (np.arange(V) % 3)    # about 2^36: neighbouring floats
+    x[5] = 2, 0
+    for qq in (q, None):
+        want = [R.verify(p[b].astype(np.float64), None if qq is None else qq[b].astype(np.float64), x[b], K, ua[b], us[b], 1.0) for b in range(B)]
+        rep = [cuda(a).repeat(times, *[1] * (a.ndim - 1)) for a in (p, x, ua, us)]
+        got = [t.view(times, B, *t.shape[1:]) for t in TK.verify_drafts(ctx, *rep, draft_logits=None if qq is None else cuda(qq).repeat(times, 1, 1))]
+        for b in range(B):
+            tok, a, lp, margin = want[b]
+            assert margin > 8 * D(V)
+            assert (got[1][:, b] == a).all() and (got[0][:, b].cpu() == torch.tensor(tok)).all(), (b, got[0][0, b], tok, got[1][0, b], a)
+            assert (got[2][:, b].cpu().double() - torch.tensor(lp)).abs().max() <= D(V) + 2 * E * max(map(abs, lp)), (b, got[2][0, b], lp)
+
+
+@pytest.mark.parametrize("u", [0.0, 1.0])
+def test_verify_chunks_of_vanishing_weight(ctx, u):
+    """Tokens of probability 2^-1010 before and behind the others are not drawn, not even by u = 0 or by the 1 that is out of range."""
+    V = 3 * 2048
+    z = np.full((1, 1, V), -700.0, np.float32)   # exp(-700) = 2^-1010
+    z[0, 0, 2100:2110] = 0.0
+    tok, acc, lp = TK.verify_drafts(ctx, cuda(z), None, None, cuda(np.array([u], np.float32)))
+    assert tok.tolist() == [[2100 if u == 0.0 else 2109]] and acc.tolist() == [0]
+    assert abs(float(lp) + math.log(10)) <= D(V) + 1e-6
+
+
 def test_verify_strides_shared_rows_and_unread_rows(ctx):
     """Logits inside a wider buffer, a target row shared by the batch (stride 0), and rows behind a sequence's drafts: not read (NaN there changes nothing)."""
     rng = np.random.default_rng(6)

@@ -37,7 +37,7 @@ VER = dict(ctx=None, target=P, dtype=2, batch=4, drafts=3, vocab=100, tb=400, tp
 
 @pytest.mark.parametrize("change, text", [
     (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 19) + 1), "vocab"), (dict(rows=-1), "rows"),
-    (dict(rows=(1 << 24) + 1), "rows"), (dict(k=0), "k 0"), (dict(k=257), "k 257"), (dict(tau=0.0), "temperature"), (dict(tau=math.nan), "temperature"),
+    (dict(rows=1 << 22), "2^22"), (dict(k=0), "k 0"), (dict(k=257), "k 257"), (dict(tau=0.0), "temperature"), (dict(tau=math.nan), "temperature"),
     (dict(tau=1e5), "temperature"), (dict(stride=99), "stride"), (dict(logits=None), "logits is null"), (dict(idx=None), "idx is null"),
     (dict(val=P + 2), "values is not aligned"), (dict(logits=P + 1), "logits is not aligned"), (dict(lse=None), "lse is null"),
     (dict(rows=1, vocab=131072, ws_bytes=16), "workspace holds 16"), (dict(rows=1, vocab=131072, ws=None), "workspace is null"), ({}, "null context"),
@@ -57,7 +57,7 @@ def test_distill_refuses(lib, change, text):
 
 @pytest.mark.parametrize("change, text", [
     (dict(dtype=9), "dtype"), (dict(batch=-1), "rows"), (dict(drafts=-1), "drafts"), (dict(drafts=129), "drafts"), (dict(tau=-0.5), "temperature"), (dict(tau=math.inf), "temperature"),
-    (dict(batch=1 << 20, drafts=100), "2^24 rows"), (dict(tp=-1), "negative stride"), (dict(db=-1), "negative stride"), (dict(target=None), "target_logits is null"),
+    (dict(batch=1 << 20, drafts=100), "2^22 rows"), (dict(tp=-1), "negative stride"), (dict(db=-1), "negative stride"), (dict(target=None), "target_logits is null"),
     (dict(tokens=None), "draft_tokens is null"), (dict(ua=None), "u_accept is null"), (dict(us=None), "u_sample is null"), (dict(draft=P + 1), "draft_logits is not aligned"),
     (dict(out=None), "tokens is null"), (dict(acc=None), "accepted is null"), (dict(vocab=50000, tp=50000, tb=1 << 20, ws_bytes=0), "workspace holds 0"),
     (dict(vocab=50000, tp=50000, tb=1 << 20, ws=P + 4), "workspace is not aligned"), ({}, "null context"), (dict(tau=0.0, ua=None, us=None, draft=None), "null context")])
