@@ -757,15 +757,18 @@ template <int DT> void top_dispatch(const TopArgs& a, const TopPlan& p, hipStrea
 // hundred, so that the row it is drawn from is summed in fp64, exponentials too.  They are 2^(z C - E), C = log2(e) / tau, with a whole number E a chunk of
 // 2048 tokens (the maximum's exponent, rounded up): sums of different chunks are brought together by exact shifts of the exponent.  An acceptance compares
 // two numbers, and sums of fp32 exponentials do for it.
+// Rows of one chunk and few drafts, one kernel:
+//   verify_one_kernel             a block a sequence: its rows' sums, then all that follows
 // Small calls, two kernels (launches are what they cost):
-//   verify_sums_kernel<true>   fp64 sums of each chunk of each row that a sequence may need (a wave a chunk), and of the chunks of a block together
-//   verify_pick_kernel<true>   acceptance, by every block of a sequence for itself; where it ends in a rejection with a draft distribution the chunks' sums of
-//                              max(p - q, 0), and the sequence's last block to finish draws the token; elsewhere its first block draws from the sums there are
+//   verify_sums_kernel<VF_SUMS>   fp64 sums of each chunk of each row that a sequence may need (a wave a chunk), and of the chunks of a block together
+//   verify_pick_kernel<VF_SUMS>   acceptance, by every block of a sequence for itself; where it ends in a rejection with a draft distribution the chunks' sums of
+//                                 max(p - q, 0), and the sequence's last block to finish draws the token; elsewhere its first block draws from the sums there are
 // Large calls, three kernels (an fp64 exponential is 20 instructions, an fp32 one with its sum 6, and but two rows a sequence need the former):
-//   verify_stats_kernel        (maximum, sum) in fp32 of the drafted positions' rows
-//   verify_sums_kernel<false>  acceptance, and the fp64 sums of the one or two rows that the token is drawn from
-//   verify_pick_kernel<false>  the rest as above
+//   verify_stats_kernel           (maximum, sum) in fp32 of the drafted positions' rows
+//   verify_sums_kernel<VF_STATS>  acceptance, and the fp64 sums of the one or two rows that the token is drawn from
+//   verify_pick_kernel<VF_STATS>  the rest as above
 constexpr int VF_T = 256, VF_WAVES = VF_T / 64, VF_CHUNK = 2048;   // 32 tokens a lane: what a chunk costs beside its exps (reductions) is shared by that many
+enum { VF_STATS, VF_SUMS, VF_ONE };          // three kernels, two, one
 struct VfSum { double e, s; };               // s 2^e; nothing: s = 0, e = -inf; a NaN among the logits: s NaN; +inf: e = +inf
 struct VerifyArgs {
   const char* target; int64_t tb, tp;        // bytes from sequence to sequence, from position to position
@@ -875,8 +878,8 @@ __global__ __launch_bounds__(VF_T) void verify_stats_kernel(VerifyArgs a) {
 }
 
 // How many drafts of sequence b are accepted; every thread of the block gets it.  srow: the rows' sums, target 0 .. n, draft 0 .. n - 1 behind them
-// (from fp32 statistics target 0 .. n - 1).  `write`: the block that writes what is known then.
-template <int DT, bool ALL> __device__ int vf_accept(const VerifyArgs& a, int b, int n, bool write, const double* table, VfSum* srow, int* sat) {
+// (from fp32 statistics target 0 .. n - 1; VF_ONE: the caller has filled them in).  `write`: the block that writes what is known then.
+template <int DT, int HOW> __device__ int vf_accept(const VerifyArgs& a, int b, int n, bool write, const double* table, VfSum* srow, int* sat) {
   const int tid = threadIdx.x;
   const int64_t k0 = (int64_t)b * a.K, t0 = (int64_t)b * (a.K + 1);
   int x = -1;
@@ -890,10 +893,10 @@ template <int DT, bool ALL> __device__ int vf_accept(const VerifyArgs& a, int b,
     }
   }
   if (tid == 0) *sat = n;
-  const int heads = ALL ? n + 1 : n, rows = heads + (a.draft ? n : 0);
+  const int heads = HOW == VF_STATS ? n : n + 1, rows = HOW == VF_ONE ? 0 : heads + (a.draft ? n : 0);
   for (int r = tid >> 4; r < rows; r += VF_T / 16) {   // 16 lanes a row
     VfSum s = {-INFINITY, 0.0};
-    if constexpr (ALL) {
+    if constexpr (HOW == VF_SUMS) {
       const VfSum* p = a.parts + (r < heads ? t0 + r : (int64_t)a.B * (a.K + 1) + k0 + r - heads) * a.nsplit;
       for (int i = tid & 15; i < a.nsplit; i += 16) s = vf_add(s, p[i]);
       for (int o = 8; o > 0; o >>= 1) s = vf_add(s, VfSum{__shfl_xor(s.e, o, 16), __shfl_xor(s.s, o, 16)});
@@ -949,9 +952,37 @@ template <int DT> __device__ __forceinline__ void vf_chunk(Pack (&y)[VF_CHUNK / 
   }
 }
 
-template <int DT, bool ALL>
-__global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
+// the fp64 sum of a wave's chunk
+template <int DT> __device__ __forceinline__ VfSum vf_sum_chunk(Pack (&x)[VF_CHUNK / 64 / Lg<DT>::VEC], int ch, const VerifyArgs& a, const double* table) {
   constexpr int VEC = Lg<DT>::VEC, U = VF_CHUNK / 64 / VEC;
+  float m = -INFINITY;
+  uint64_t nan = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    m = fmaxf(m, tk_max<DT>(x[u]));
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) nan |= __ballot(__builtin_isunordered(tk_get<DT>(x[u], j), tk_get<DT>(x[u], j + 1)));
+  }
+  m = wave_max(m);
+  const double E = vf_ceil(a, m);
+  const VfExp ex = {table, 32.0 * vf_slope(a, E), 32.0 * E};
+  double s = 0.0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if ((ch * U + u) * 64 * VEC >= a.V) break;   // (the same for every lane)
+    tk_redecode(x[u]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s += ex(tk_get<DT>(x[u], j));
+  }
+  s = wave_sum(s);
+  if (m == -INFINITY) s = 0.0;
+  if (nan) s = NAN;
+  return VfSum{m == -INFINITY ? -INFINITY : E, s};
+}
+
+template <int DT, int HOW>
+__global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
+  constexpr int U = VF_CHUNK / 64 / Lg<DT>::VEC;
   __shared__ double table[32];
   __shared__ VfSum part[VF_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -959,7 +990,7 @@ __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
   const int split = (int)(blockIdx.x % (uint32_t)a.nsplit);
   const char* z;
   if (tid < 32) table[tid] = exp2(tid / 32.0);
-  if constexpr (ALL) {
+  if constexpr (HOW == VF_SUMS) {
     const int64_t trows = (int64_t)a.B * (a.K + 1);
     if (row < trows) {
       const int b = (int)(row / (a.K + 1)), i = (int)(row - (int64_t)b * (a.K + 1));
@@ -976,7 +1007,7 @@ __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
     __shared__ int sat;
     const bool of_draft = row >= a.B;
     const int b = (int)(of_draft ? row - a.B : row), n = vf_drafts(a, b);
-    const int at = vf_accept<DT, false>(a, b, n, !of_draft && split == 0, table, srow, &sat);
+    const int at = vf_accept<DT, VF_STATS>(a, b, n, !of_draft && split == 0, table, srow, &sat);
     if (!of_draft && split == 0 && tid == 0) a.done[b] = 0;
     if (of_draft && at >= n) return;
     z = of_draft ? a.draft + b * a.db + at * a.dp : a.target + b * a.tb + at * a.tp;
@@ -991,29 +1022,7 @@ __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) x[u] = y[u];
     if (ch + VF_WAVES < c1) vf_chunk<DT>(y, z, ch + VF_WAVES, a.V);
-    float m = -INFINITY;
-    uint64_t nan = 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      m = fmaxf(m, tk_max<DT>(x[u]));
-#pragma unroll
-      for (int j = 0; j < VEC; j += 2) nan |= __ballot(__builtin_isunordered(tk_get<DT>(x[u], j), tk_get<DT>(x[u], j + 1)));
-    }
-    m = wave_max(m);
-    const double E = vf_ceil(a, m);
-    const VfExp ex = {table, 32.0 * vf_slope(a, E), 32.0 * E};
-    double s = 0.0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if ((ch * U + u) * 64 * VEC >= a.V) break;   // (the same for every lane)
-      tk_redecode(x[u]);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) s += ex(tk_get<DT>(x[u], j));
-    }
-    s = wave_sum(s);
-    if (m == -INFINITY) s = 0.0;
-    if (nan) s = NAN;
-    const VfSum mine = {m == -INFINITY ? -INFINITY : E, s};
+    const VfSum mine = vf_sum_chunk<DT>(x, ch, a, table);
     if (lane == 0) a.sums[row * a.nchunk + ch] = mine;
     all = vf_add(all, mine);
   }
@@ -1039,12 +1048,66 @@ __device__ double vf_scan(double v, double* ss, double* total) {
   return v;
 }
 
-template <int DT, bool ALL>
+// What a token weighs in the draw: p, max(p - q, 0) where there is a draft row, or p but for one token
+template <int DT> struct VfWeight {
+  const char *prow, *qrow;
+  VfExp ep, eq;
+  double np, nq, none;
+  int V, skip;
+  __device__ __forceinline__ VfWeight(const VerifyArgs& a, const double* table, const char* prow, const VfSum& ps, const char* qrow, const VfSum& qs)
+    : prow(prow), qrow(qrow), ep{table, 32.0 * vf_slope(a, ps.e), 32.0 * ps.e}, eq{table, 32.0 * vf_slope(a, qs.e), 32.0 * qs.e}, np(1.0 / ps.s), nq(1.0 / qs.s),
+      none(2.0 * VF_NOTHING * np), V(a.V), skip(-1) {}
+  __device__ __forceinline__ void leave_out(int token) { if ((uint32_t)token < (uint32_t)V) skip = token; }   // a looked-up token that was rejected
+  __device__ __forceinline__ bool less() const { return qrow || skip >= 0; }
+  __device__ __forceinline__ void p_itself() { qrow = nullptr; skip = -1; }
+  __device__ __forceinline__ double rest(float zp, float zq) const { return fmax(fma(ep(zp), np, fma(eq(zq), -nq, -none)), 0.0); }
+  __device__ __forceinline__ double operator()(int e) const {
+    if (e >= V || e == skip) return 0.0;
+    const float zp = tk_at<DT>(prow, e);
+    return qrow ? rest(zp, tk_at<DT>(qrow, e)) : fmax(fma(ep(zp), np, -none), 0.0);
+  }
+};
+
+// Draws a token among the chunk from token c0 on, `below` of the weight lying before it: the first whose cumulative weight exceeds `goal` (negative: the
+// chunk is all there is, the goal goes by its weight; false if it has none and could have more); rounding, or u >= 1, may leave none: the last of any weight.
+template <int DT> __device__ bool vf_token(const VerifyArgs& a, int64_t o, const VfWeight<DT>& weight, const VfSum& ps, const char* prow, int c0, double below, double goal,
+                                           double* ss, int* sfirst, int* slast) {
+  constexpr int PER = VF_CHUNK / VF_T;
+  const int e0 = c0 + threadIdx.x * PER;
+  double t[PER], s = 0.0, sum;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) { t[j] = weight(e0 + j); s += t[j]; }
+  double c = below + (vf_scan(s, ss, &sum) - s);
+  if (goal < 0.0) {
+    if (!(sum > 0.0) && weight.less()) return false;
+    const float u = a.u_sample[o / (a.K + 1)];
+    goal = (u > 0.0f ? (double)u : 0.0) * sum;
+  }
+  if (threadIdx.x == 0) { *sfirst = a.V; *slast = -1; }
+  __syncthreads();
+  int first = a.V, last = -1;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    c += t[j];
+    if (t[j] > 0.0) { last = e0 + j; if (c > goal && first == a.V) first = last; }
+  }
+  if (first < a.V) atomicMin(sfirst, first);
+  if (last >= 0) atomicMax(slast, last);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int token = *sfirst < a.V ? *sfirst : *slast;
+    a.out[o] = token;
+    if (a.logprobs) a.logprobs[o] = (float)vf_logp(a, ps, tk_at<DT>(prow, token));
+  }
+  return true;
+}
+
+template <int DT, int HOW>
 __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
   constexpr int VEC = Lg<DT>::VEC, U = VF_CHUNK / 64 / VEC;
   __shared__ double table[32];
   __shared__ double ss[VF_WAVES];
-  __shared__ VfSum srow[ALL ? 2 * TK_MAX_DRAFTS + 1 : 2];
+  __shared__ VfSum srow[HOW == VF_STATS ? 2 : 2 * TK_MAX_DRAFTS + 1];
   __shared__ int sat, sfirst, slast, slastblock;
   __shared__ double sbelow;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1053,8 +1116,8 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
   if (tid < 32) table[tid] = exp2(tid / 32.0);
   int at, prow_at, qrow_at;                  // drafts accepted; where srow holds the row that the token is drawn from, and the draft's
   int64_t prow_id;                           // which row of `sums` it is
-  if constexpr (ALL) {
-    at = vf_accept<DT, true>(a, b, n, part == 0, table, srow, &sat);
+  if constexpr (HOW == VF_SUMS) {
+    at = vf_accept<DT, VF_SUMS>(a, b, n, part == 0, table, srow, &sat);
     prow_at = at; qrow_at = n + 1 + at;
     prow_id = (int64_t)b * (a.K + 1) + at;
   } else {
@@ -1079,10 +1142,8 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
   const char* prow = a.target + b * a.tb + at * a.tp;
   const char* qrow = a.draft && at < n && vf_good(srow[qrow_at]) ? a.draft + b * a.db + at * a.dp : nullptr;
   const VfSum qs = qrow ? srow[qrow_at] : VfSum{0.0, 1.0};
-  const VfExp ep = {table, 32.0 * vf_slope(a, ps.e), 32.0 * ps.e}, eq = {table, 32.0 * vf_slope(a, qs.e), 32.0 * qs.e};
-  const double np = 1.0 / ps.s, nq = 1.0 / qs.s, none = 2.0 * VF_NOTHING * np;
-  bool rest = qrow != nullptr;
-  if (rest) {
+  VfWeight<DT> weight(a, table, prow, ps, qrow, qs);
+  if (qrow) {
     for (int ch = part * VF_WAVES + wave; ch < a.nchunk; ch += a.npick * VF_WAVES) {
       Pack px[U], qx[U];
       vf_chunk<DT>(px, prow, ch, a.V);
@@ -1092,7 +1153,7 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
       for (int u = 0; u < U; ++u) {
         if ((ch * U + u) * 64 * VEC >= a.V) break;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s += fmax(fma(ep(tk_get<DT>(px[u], j)), np, fma(eq(tk_get<DT>(qx[u], j)), -nq, -none)), 0.0);
+        for (int j = 0; j < VEC; ++j) s += weight.rest(tk_get<DT>(px[u], j), tk_get<DT>(qx[u], j));
       }
       s = wave_sum(s);
       if (lane == 0) __hip_atomic_store(&a.rest[(int64_t)b * a.nchunk + ch], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1108,18 +1169,14 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
   } else if (part != 0) return;
 
   // the chunk that the goal falls into; a thread looks at neighbouring chunks
-  const int rejected = !a.draft && at < n ? a.tokens[(int64_t)b * a.K + at] : -1;
-  int skip = (uint32_t)rejected < (uint32_t)a.V ? rejected : -1;   // a looked-up token that was rejected has no weight left
-  const auto weight = [&](int e) {
-    if (e >= a.V || e == skip) return 0.0;
-    return fmax(fma(ep(tk_at<DT>(prow, e)), np, rest ? fma(eq(tk_at<DT>(qrow, e)), -nq, -none) : -none), 0.0);
-  };
+  if (!a.draft && at < n) weight.leave_out(a.tokens[(int64_t)b * a.K + at]);
   const VfSum* sums = a.sums + prow_id * a.nchunk;
   const int per = (a.nchunk + VF_T - 1) / VF_T;
   const float u = a.u_sample[b];
   double total, goal, before;
   for (;;) {
     double without = 0.0;                    // the skipped token's chunk, summed again without it
+    const int skip = weight.skip;
     if (skip >= 0) {
       double w = 0.0;
       for (int j = 0; j < VF_CHUNK / VF_T; ++j) w += weight(skip / VF_CHUNK * VF_CHUNK + tid * (VF_CHUNK / VF_T) + j);
@@ -1127,15 +1184,15 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
     }
     const auto chunk = [&](int i) {
       if (i >= a.nchunk) return 0.0;
-      if (rest) return (double)__hip_atomic_load(&a.rest[(int64_t)b * a.nchunk + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (weight.qrow) return (double)__hip_atomic_load(&a.rest[(int64_t)b * a.nchunk + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       if (skip >= 0 && i == skip / VF_CHUNK) return without;
       // a chunk that counts has a token that counts: its largest is above 2^-991 of the row's, and weight() leaves out what is below 2^-999
-      return sums[i].e - ps.e >= -990.0 ? vf_scaled(sums[i], ps.e) * np : 0.0;
+      return sums[i].e - ps.e >= -990.0 ? vf_scaled(sums[i], ps.e) * weight.np : 0.0;
     };
     double mine = 0.0;
     for (int j = 0; j < per; ++j) mine += chunk(tid * per + j);
     before = vf_scan(mine, ss, &total) - mine;
-    if (!(total > 0.0) && (rest || skip >= 0)) { rest = false; skip = -1; continue; }   // nothing left of p: p itself
+    if (!(total > 0.0) && weight.less()) { weight.p_itself(); continue; }   // nothing left of p
     if (tid == 0) { sfirst = a.nchunk; slast = -1; }
     __syncthreads();
     goal = (u > 0.0f ? (double)u : 0.0) * total;
@@ -1152,31 +1209,66 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
     const int hit = sfirst < a.nchunk ? sfirst : slast;   // (rounding, or u >= 1, may leave no sum above the goal: the last weight there is)
     if (hit / per == tid) { c = before; for (int j = tid * per; j < hit; ++j) c += chunk(j); sbelow = c; }
     __syncthreads();
-    // the token inside the chunk
-    constexpr int PER = VF_CHUNK / VF_T;
-    const int e0 = hit * VF_CHUNK + tid * PER;
-    double t[PER], s = 0.0, sum;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) { t[j] = weight(e0 + j); s += t[j]; }
-    c = sbelow + (vf_scan(s, ss, &sum) - s);
-    if (tid == 0) { sfirst = a.V; slast = -1; }
-    __syncthreads();
-    first = a.V; last = -1;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      c += t[j];
-      if (t[j] > 0.0) { last = e0 + j; if (c > goal && first == a.V) first = last; }
-    }
-    if (first < a.V) atomicMin(&sfirst, first);
-    if (last >= 0) atomicMax(&slast, last);
-    __syncthreads();
+    vf_token<DT>(a, o, weight, ps, prow, hit * VF_CHUNK, sbelow, goal, ss, &sfirst, &slast);
     break;
   }
-  if (tid == 0) {
-    const int token = sfirst < a.V ? sfirst : slast;
-    a.out[o] = token;
-    if (a.logprobs) a.logprobs[o] = (float)vf_logp(a, ps, tk_at<DT>(prow, token));
+}
+
+// Rows of one chunk and few of them: a block a sequence.  Up to 16 lanes' vectors: 16 rows at once, else a wave a row.  The weights of the row that is
+// drawn from are looked at once.
+template <int DT>
+__global__ __launch_bounds__(VF_T, 4) void verify_one_kernel(VerifyArgs a) {
+  constexpr int VEC = Lg<DT>::VEC, U = VF_CHUNK / 64 / VEC;
+  __shared__ double table[32];
+  __shared__ double ss[VF_WAVES];
+  __shared__ VfSum srow[2 * TK_MAX_DRAFTS + 1];
+  __shared__ int sat, sfirst, slast;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = (int)blockIdx.x, n = vf_drafts(a, b), rows = n + 1 + (a.draft ? n : 0);
+  const auto at_row = [&](int r) { return r <= n ? a.target + b * a.tb + r * a.tp : a.draft + b * a.db + (r - n - 1) * a.dp; };
+  if (tid < 32) table[tid] = exp2(tid / 32.0);
+  __syncthreads();
+  if (a.V <= 16 * VEC) {
+    for (int r = tid >> 4; r < rows; r += VF_T / 16) {
+      const Pack x = tk_load<DT>(at_row(r), tid & 15, a.V);
+      float m = tk_max<DT>(x);
+      bool nan = false;
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) nan |= __builtin_isunordered(tk_get<DT>(x, j), tk_get<DT>(x, j + 1));
+      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
+      const double E = vf_ceil(a, m);
+      const VfExp ex = {table, 32.0 * vf_slope(a, E), 32.0 * E};
+      double s = 0.0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s += ex(tk_get<DT>(x, j));
+      if (m == -INFINITY) s = 0.0;
+      if (nan) s = NAN;
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
+      if ((tid & 15) == 0) srow[r] = VfSum{m == -INFINITY ? -INFINITY : E, s};
+    }
+  } else {
+    Pack y[U];
+    if (wave < rows) vf_chunk<DT>(y, at_row(wave), 0, a.V);
+    for (int r = wave; r < rows; r += VF_WAVES) {
+      Pack x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = y[u];
+      if (r + VF_WAVES < rows) vf_chunk<DT>(y, at_row(r + VF_WAVES), 0, a.V);
+      const VfSum sum = vf_sum_chunk<DT>(x, 0, a, table);
+      if (lane == 0) srow[r] = sum;
+    }
   }
+  const int at = vf_accept<DT, VF_ONE>(a, b, n, true, table, srow, &sat);
+  const int64_t o = (int64_t)b * (a.K + 1) + at;
+  const VfSum ps = srow[at];
+  if (!vf_good(ps)) {
+    if (tid == 0) { a.out[o] = -1; if (a.logprobs) a.logprobs[o] = 0.0f; }
+    return;
+  }
+  const bool less = a.draft && at < n && vf_good(srow[n + 1 + at]);
+  VfWeight<DT> weight(a, table, at_row(at), ps, less ? at_row(n + 1 + at) : nullptr, less ? srow[n + 1 + at] : VfSum{0.0, 1.0});
+  if (!a.draft && at < n) weight.leave_out(a.tokens[(int64_t)b * a.K + at]);
+  while (!vf_token<DT>(a, o, weight, ps, at_row(at), 0, 0.0, -1.0, ss, &sfirst, &slast)) weight.p_itself();
 }
 
 // tau = 0: p is one-hot at the row's largest logit (the lowest index of equal ones), a draft is accepted where it is that token
@@ -1244,20 +1336,25 @@ __global__ __launch_bounds__(VF_T) void verify_greedy_kernel(VerifyArgs a) {
   if (tid == 0) a.accepted[b] = sa;
 }
 
-struct VerifyPlan { bool all; int nchunk, nstat, nsplit, npick; size_t o_parts, o_rest, o_stats, o_done, ws; };
-VerifyPlan verify_plan(int B, int K, int V, bool draft, bool greedy) {
+struct VerifyPlan { int how, nchunk, nstat, nsplit, npick; size_t o_parts, o_rest, o_stats, o_done, ws; };
+VerifyPlan verify_plan(int dtype, int B, int K, int V, bool draft, bool greedy) {
   VerifyPlan p = {};
   p.nchunk = (V + VF_CHUNK - 1) / VF_CHUNK;
+  // One kernel saves a launch, the workspace and the blocks' own acceptance, but has four waves for all rows of a sequence: us of the GPU, one / two kernels,
+  // fp32 with draft logits: 18 tokens: 120 sequences of 7 drafts 8 / 19, 1000 of 128 31 / 854, one of 128 20 / 26;  300 tokens: one sequence of 3 drafts
+  // 12 / 17, of 16 25 / 19, 120 of 16 26 / 30, of 40 46 / 49;  2048 tokens: one of 3 17 / 17, of 7 21 / 17, 120 of 16 37 / 37, of 40 67 / 50, 1000 of 128 496 / 634
+  const int own = K + 1 + (draft ? K : 0);
+  if (!greedy && p.nchunk == 1 && (V <= 16 * (dtype == CBM_F32 ? 4 : 8) || own <= 12 || 3 * own <= B)) { p.how = VF_ONE; return p; }
   const int64_t all = (int64_t)B * (K + 1) + (draft && !greedy ? (int64_t)B * K : 0);
   // fp64 sums of every row up to 2^24 logits (about 12 us of fp64 beside a launch saved of 5); beyond, of the rows that tokens are drawn from
-  p.all = greedy || K == 0 || all * V <= (1 << 24);
-  const int64_t rows = p.all ? all : (int64_t)B * (draft ? 2 : 1);
+  p.how = greedy || K == 0 || all * V <= (1 << 24) ? VF_SUMS : VF_STATS;
+  const int64_t rows = p.how == VF_SUMS ? all : (int64_t)B * (draft ? 2 : 1);
   const int most = (p.nchunk + VF_WAVES - 1) / VF_WAVES;   // a chunk a wave
   // blocks: about 16384 of the fp64 sums, 1024 in the last kernel, 8192 of the fp32 statistics
   const auto share = [](int64_t blocks, int64_t of, int most) { const int64_t n = (blocks + of - 1) / of; return (int)(n < most ? n : most); };
   p.nsplit = share(16384, rows, most);
   p.npick = draft && K > 0 ? share(1024, B, most) : 1;
-  p.nstat = p.all ? 0 : share(8192, all, (V + 8191) / 8192);
+  p.nstat = p.how == VF_SUMS ? 0 : share(8192, all, (V + 8191) / 8192);
   if (greedy) { p.ws = (size_t)rows * p.nsplit * sizeof(VfBest); return p; }
   p.o_parts = (size_t)rows * p.nchunk * sizeof(VfSum);
   p.o_rest = p.o_parts + (size_t)rows * p.nsplit * sizeof(VfSum);
@@ -1272,14 +1369,17 @@ template <int DT> void verify_dispatch(const VerifyArgs& a, const VerifyPlan& p,
     hipLaunchKernelGGL(verify_greedy_kernel, dim3(a.B), dim3(VF_T), 0, st, a);
     return;
   }
-  const int64_t rows = (int64_t)a.B * (p.all ? a.K + 1 : 1) + (a.draft ? (int64_t)a.B * (p.all ? a.K : 1) : 0);
-  if (p.all) {
-    hipLaunchKernelGGL((verify_sums_kernel<DT, true>), dim3((uint32_t)(rows * a.nsplit)), dim3(VF_T), 0, st, a);
-    hipLaunchKernelGGL((verify_pick_kernel<DT, true>), dim3((uint32_t)a.B * a.npick), dim3(VF_T), 0, st, a);
+  if (p.how == VF_ONE) {
+    hipLaunchKernelGGL(verify_one_kernel<DT>, dim3(a.B), dim3(VF_T), 0, st, a);
+  } else if (p.how == VF_SUMS) {
+    const int64_t rows = (int64_t)a.B * (a.K + 1) + (a.draft ? (int64_t)a.B * a.K : 0);
+    hipLaunchKernelGGL((verify_sums_kernel<DT, VF_SUMS>), dim3((uint32_t)(rows * a.nsplit)), dim3(VF_T), 0, st, a);
+    hipLaunchKernelGGL((verify_pick_kernel<DT, VF_SUMS>), dim3((uint32_t)a.B * a.npick), dim3(VF_T), 0, st, a);
   } else {
-    hipLaunchKernelGGL(verify_stats_kernel<DT>, dim3((uint32_t)((int64_t)a.B * a.K * (a.draft ? 2 : 1) * a.nstat)), dim3(VF_T), 0, st, a);
-    hipLaunchKernelGGL((verify_sums_kernel<DT, false>), dim3((uint32_t)(rows * a.nsplit)), dim3(VF_T), 0, st, a);
-    hipLaunchKernelGGL((verify_pick_kernel<DT, false>), dim3((uint32_t)a.B * a.npick), dim3(VF_T), 0, st, a);
+    const int64_t rows = (int64_t)a.B * (a.draft ? 2 : 1);
+    hipLaunchKernelGGL(verify_stats_kernel<DT>, dim3((uint32_t)(rows * a.K * a.nstat)), dim3(VF_T), 0, st, a);
+    hipLaunchKernelGGL((verify_sums_kernel<DT, VF_STATS>), dim3((uint32_t)(rows * a.nsplit)), dim3(VF_T), 0, st, a);
+    hipLaunchKernelGGL((verify_pick_kernel<DT, VF_STATS>), dim3((uint32_t)a.B * a.npick), dim3(VF_T), 0, st, a);
   }
 }
 
@@ -1401,7 +1501,7 @@ static int verify_check(const char* fn, int dtype, int B, int K, int V, double t
 }
 extern "C" int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, double temperature) {
   if (verify_check("cbm_verify_drafts_workspace", dtype, batch, drafts, vocab, temperature)) return -1;
-  return batch ? (int64_t)verify_plan(batch, drafts, vocab, with_draft_logits != 0, temperature == 0.0).ws : 0;
+  return batch ? (int64_t)verify_plan(dtype, batch, drafts, vocab, with_draft_logits != 0, temperature == 0.0).ws : 0;
 }
 extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab,
                                  int64_t target_batch_stride, int64_t target_pos_stride, const void* draft_logits, int64_t draft_batch_stride,
@@ -1421,7 +1521,7 @@ extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t 
   if (!greedy && tk_pointer(fn, "u_sample", u_sample, 4)) return -1;
   if (draft_logits && tk_pointer(fn, "draft_logits", draft_logits, es)) return -1;
   if (drafts == 0 || greedy) draft_logits = nullptr;   // (not looked at)
-  const VerifyPlan p = verify_plan(batch, drafts, vocab, draft_logits != nullptr, greedy);
+  const VerifyPlan p = verify_plan(dtype, batch, drafts, vocab, draft_logits != nullptr, greedy);
   if (tk_workspace(fn, workspace, workspace_bytes, p.ws)) return -1;
   if (!c) TK_REFUSE("%s: null context", fn);
   DeviceScope dev(c);

@@ -308,7 +308,7 @@ def check_verify(ctx, p, tp, q, tq, x, n, ua, us, tau):
 
 @pytest.mark.parametrize("looked_up, ragged", [(False, False), (False, True), (True, True)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("B, K, V", [(1, 1, 1), (3, 2, 2), (120, 7, 18), (5, 128, 33), (4, 3, 1000), (6, 0, 5000), (3, 5, 4096), (5, 4, 4097), (2, 6, 50021), (1, 4, 131072), (1, 1, 524288)])
+@pytest.mark.parametrize("B, K, V", [(1, 1, 1), (3, 2, 2), (120, 7, 18), (5, 128, 33), (4, 3, 1000), (120, 7, 65), (9, 4, 64), (5, 30, 300), (70, 2, 2048), (2, 3, 129), (6, 0, 5000), (3, 5, 4096), (5, 4, 4097), (2, 6, 50021), (1, 4, 131072), (1, 1, 524288)])
 def test_verify_drafts(ctx, dtype, B, K, V, looked_up, ragged):
     rng = np.random.default_rng(B * 1000 + V + K)
     tau = 1.0 if B % 2 else 0.8
