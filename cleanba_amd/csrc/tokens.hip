@@ -179,7 +179,7 @@ template <int DT, int T, int NV, bool TAIL>
 __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   constexpr int VEC = Lg<DT>::VEC, ES = Lg<DT>::ES, U = 4;
   __shared__ MS red[T / 64];
-  __shared__ int32_t sidx[TK_MAX_TOP];
+  __shared__ __align__(16) int32_t sidx[TK_MAX_TOP];
   __shared__ float sz[TK_MAX_TOP], sv[TK_MAX_TOP];     // the student's and the teacher's logits there
   __shared__ double st[TK_MAX_TOP], slt[TK_MAX_TOP];   // t_k and log t_k
   __shared__ uint8_t ssame[TK_MAX_TOP];      // 0: not the first slot of its token (or empty), 1: its only one, 2: the first of several
@@ -224,13 +224,18 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
   if ((uint32_t)my >= (uint32_t)V) my = -1;  // -1 and whatever lies outside the vocabulary: an empty slot
   if (my >= 0) myz = tk_at<DT>(row0, my);
   if (tid < K) { sidx[tid] = my; sz[tid] = myz; sv[tid] = my >= 0 ? myv : -INFINITY; }
+  else if (tid < ((K + 3) & ~3)) sidx[tid] = -2;
   if constexpr (TAIL) for (int i = tid; i < (V + 31) / 32 + 1; i += T) bits[i] = 0;
   __syncthreads();
   if (tid < K) {
-    int same = 0;
-    bool first = my >= 0;
-    for (int j = 0; j < K; ++j) if (sidx[j] == my) { ++same; first = first && j >= tid; }
-    ssame[tid] = !first ? 0 : (same == 1 ? 1 : 2);
+    int same = 0, low = K;                   // how many slots hold the token, the first of them
+    for (int j = 0; j < K; j += 4) {
+      const int4 of = *reinterpret_cast<const int4*>(sidx + j);
+      const uint32_t is = (of.x == my ? 1u : 0u) | (of.y == my ? 2u : 0u) | (of.z == my ? 4u : 0u) | (of.w == my ? 8u : 0u);
+      same += __popc(is);
+      low = min(low, is ? j + (int)__builtin_ctz(is | 16u) : K);
+    }
+    ssame[tid] = my < 0 || low != tid ? 0 : (same == 1 ? 1 : 2);
     if constexpr (TAIL) if (my >= 0) atomicOr(&bits[my >> 5], 1u << (my & 31));
   }
   if constexpr (TAIL) __syncthreads();

@@ -20,6 +20,7 @@ import torch
 from . import lib as L
 
 _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+# (new_empty of a tensor of the right type is quicker than empty by 0.3 us)
 _empty, _i32, _f32, _u8 = torch.empty, torch.int32, torch.float32, torch.uint8
 try:   # the handle alone: a Stream object costs 2 us, as much as the launch
     _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -100,7 +101,7 @@ def top_logits(ctx, logits, k, temperature=1.0):
     ws = _empty((nbytes,), dtype=_u8, device=dev) if nbytes else None   # (held to the end of the call; behind it the allocator hands it out in stream order)
     idx = _empty(lead + (k,), dtype=_i32, device=dev)
     values = _empty(lead + (k,), dtype=_f32, device=dev)
-    lse = _empty(lead, dtype=_f32, device=dev)
+    lse = values.new_empty(lead)
     if ctx.lib.cbm_top_logits(ctx.h, logits.data_ptr(), dtype, rows, vocab, stride, k, temperature, idx.data_ptr(), values.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes,
                               _raw_stream(index)):
         L._chk(-1)
@@ -116,7 +117,7 @@ def distill_loss_grad(ctx, logits, teacher_idx, teacher_logits, teacher_lse=None
     index = ctx.cfg.device
     dtype, shape, strides = _logits(index, logits, "logits")
     rows, stride = _rows(logits, shape, strides, "logits")
-    vocab, lead, dev = shape[-1], shape[:-1], logits.device
+    vocab, lead = shape[-1], shape[:-1]
     if not isinstance(teacher_idx, torch.Tensor) or teacher_idx.dim() != len(shape):
         raise ValueError(f"teacher_idx: an int32 tensor of shape {tuple(lead) + ('k',)} is expected")
     k = teacher_idx.shape[-1]
@@ -127,10 +128,10 @@ def distill_loss_grad(ctx, logits, teacher_idx, teacher_logits, teacher_lse=None
         teacher_lse = _operand(index, teacher_lse, "teacher_lse", _f32, lead)
     if row_weight is not None:
         row_weight = _operand(index, row_weight, "row_weight", _f32, lead)
-    loss = _empty(lead, dtype=_f32, device=dev)
+    loss = teacher_logits.new_empty(lead)
     grad, gstride = None, 0
     if want_grad:
-        grad, gstride = (logits, stride) if in_place else (_empty(shape, dtype=logits.dtype, device=dev), vocab)
+        grad, gstride = (logits, stride) if in_place else (logits.new_empty(shape), vocab)
     if ctx.lib.cbm_distill_loss_grad(ctx.h, logits.data_ptr(), dtype, rows, vocab, stride, teacher_idx.data_ptr(), teacher_logits.data_ptr(), k,
                                      _ptr(teacher_lse), _ptr(row_weight), temperature, loss.data_ptr(), _ptr(grad), gstride, _raw_stream(index)):
         L._chk(-1)
@@ -170,7 +171,7 @@ def verify_drafts(ctx, target_logits, draft_tokens, u_accept, u_sample, draft_lo
     nbytes = _verify_workspace(dtype, batch, drafts, vocab, draft_logits is not None, temperature)
     ws = _empty((nbytes,), dtype=_u8, device=dev) if nbytes else None   # (held to the end of the call; behind it the allocator hands it out in stream order)
     tokens = _empty((batch, positions), dtype=_i32, device=dev)
-    accepted = _empty((batch,), dtype=_i32, device=dev)
+    accepted = tokens.new_empty((batch,))
     logprobs = _empty((batch, positions), dtype=_f32, device=dev)
     if ctx.lib.cbm_verify_drafts(ctx.h, target_logits.data_ptr(), dtype, batch, drafts, vocab, tstride[0], tstride[1], _ptr(draft_logits), dstride[0], dstride[1],
                                  _ptr(draft_tokens), _ptr(n_draft), _ptr(u_accept), _ptr(u_sample), temperature, tokens.data_ptr(), accepted.data_ptr(),
