@@ -399,6 +399,8 @@ template <int DT>
 void distill_dispatch(const DistillArgs& a, hipStream_t st) {
   const int nv = (a.V + Lg<DT>::VEC - 1) / Lg<DT>::VEC;
   if (nv <= 64 && a.K <= 64) distill_launch<DT, 64, 1>(a, st);
+  else if (nv <= 256 && a.K <= 64) distill_launch<DT, 64, 4>(a, st);
+  else if (nv <= 512 && a.K <= 128) distill_launch<DT, 128, 4>(a, st);
   else if (nv <= 10 * 256) distill_launch<DT, 256, 8>(a, st);
   else if (nv <= 20 * 512) distill_launch<DT, 512, 8>(a, st);
   else distill_launch<DT, 1024, 8>(a, st);
@@ -486,8 +488,13 @@ template <int T> __device__ void top_write(const uint64_t* buf, int n, int K, in
   const int live = __syncthreads_count(mine != 0);
   if (mine) {
     int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += buf[j] > mine;
+    int j = 0;
+#pragma unroll 2
+    for (; j + 4 <= n; j += 4) {
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(buf + j), y = *reinterpret_cast<const ulonglong2*>(buf + j + 2);
+      rank += (x.x > mine) + (x.y > mine) + (y.x > mine) + (y.y > mine);
+    }
+    for (; j < n; ++j) rank += buf[j] > mine;
     if (rank < K) {
       if (keys) keys[rank] = mine;
       else { idx[rank] = top_index(mine); val[rank] = top_value(top_order_of(mine)); }
@@ -516,7 +523,7 @@ template <int DT, int T, int U> __device__ __forceinline__ void top_chunk(Pack (
 template <int DT, int T, int EPT, int G, int MOST>
 __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
   constexpr int VEC = Lg<DT>::VEC, U = EPT / VEC;
-  extern __shared__ uint64_t buf[];          // [cap]
+  extern __shared__ __align__(16) uint64_t buf[];          // [cap]
   __shared__ TopShared<T> sh;
   __shared__ MS red[T / 64];
   __shared__ int sfull[3];                   // whether a chunk's elements found no room: one a pass, in turn
@@ -669,7 +676,7 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
 // the splits of a row: their keys are one more buffer to cut
 template <int T, int MOST>
 __global__ __launch_bounds__(T) void top_join_kernel(TopArgs a) {
-  extern __shared__ uint64_t buf[];
+  extern __shared__ __align__(16) uint64_t buf[];
   __shared__ TopShared<T> sh;
   const int tid = threadIdx.x, K = a.K, n = a.nsplit * K;
   const int64_t r = blockIdx.x;
