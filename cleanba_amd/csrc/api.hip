@@ -516,11 +516,22 @@ extern "C" int cbm_actor_step_async(cbm_ctx* c, int32_t s, const uint8_t* obs, c
 extern "C" int cbm_host_register(cbm_ctx* c, void* ptr, int64_t nbytes) {
   CBM_HIP(hipSetDevice(c->cfg.device));
   if (!ptr || nbytes <= 0) { cbm_set_error("cbm_host_register: empty buffer"); return -1; }
-  CBM_HIP(hipHostRegister(ptr, (size_t)nbytes, hipHostRegisterDefault));
+  const hipError_t e = hipHostRegister(ptr, (size_t)nbytes, hipHostRegisterDefault);
+  if (e == hipErrorInvalidValue || e == hipErrorNotSupported) {   // a system that page-locks no existing memory: staged copies, same results
+    (void)hipGetLastError();                 // (or the next call's check reports it)
+    std::lock_guard<std::mutex> lk(c->pageable_mu);
+    c->pageable.insert(ptr);
+    return 0;
+  }
+  CBM_HIP(e);
   return 0;
 }
 extern "C" int cbm_host_unregister(cbm_ctx* c, void* ptr) {
   CBM_HIP(hipSetDevice(c->cfg.device));
+  {
+    std::lock_guard<std::mutex> lk(c->pageable_mu);
+    if (c->pageable.erase(ptr)) return 0;
+  }
   CBM_HIP(hipHostUnregister(ptr));
   return 0;
 }

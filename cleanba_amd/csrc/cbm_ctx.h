@@ -2,6 +2,7 @@
 #pragma once
 #include "cbm_internal.h"
 #include <mutex>
+#include <set>
 #include <condition_variable>
 #include <atomic>
 #include <vector>
@@ -102,6 +103,8 @@ struct cbm_ctx {
   size_t win_bytes[CBM_WINDOWS] = {0, 0};
   bool win_fine[CBM_WINDOWS] = {false, false};
   std::mutex maps_mu;
+  std::mutex pageable_mu;
+  std::set<void*> pageable;                  // host buffers whose page-locking the system refused
   std::vector<void*> maps;   // peer windows this context opened with cbm_ipc_open_window (closed by cbm_ipc_close_all / destroy)
 };
 // publish: store the sequence number (release), then wake the sleepers
