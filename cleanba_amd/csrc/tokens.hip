@@ -143,9 +143,15 @@ template <int T> __device__ __forceinline__ MS block_lse(float m, float s, float
 //   loss  = w tau^2 [ sum_k t_k (log t_k - log s_{i_k}) + t_T (log t_T - log s_T) ]
 //   dz_j  = w tau   [ s_j (sum_k t_k + t_T) - sum_{k: i_k = j} t_k - [j outside top] t_T s_j / s_T ]
 // A block takes a row at a time.  The row's first NV vectors a thread stay in registers, so that the logits are read once for statistics and gradient;
-// what lies behind them is read twice.  With a tail, a bitmap of the top tokens keeps them out of the streamed sum: s_T is then a sum of its own with a maximum of its own, not a difference that cancels, and the top tokens join it from the wave that holds the
-// teacher.  Every other token's gradient is one coefficient times an exponential; the top tokens' gradients are stored last, over what the stream left.
+// what lies behind them is read twice.  With a tail, a bitmap of the top tokens keeps them out of the streamed sum: s_T is then a sum of its own with a
+// maximum of its own, not a difference that cancels, and the top tokens join it from the wave that holds the teacher.  Every other token's gradient is
+// one coefficient times an exponential; the top tokens' gradients are stored last, over what the stream left.
 // log2(e) / tau is rounded to fp32 once and used so throughout the student's side, loss included: the loss of a temperature off by 6e-8.
+// Bound by memory where there are rows enough: 3840 rows of 131072 bf16, K 64, 427 us = 4.7 TB/s of one reading and one writing (a large copy reaches 4.85);
+// 777 rows of 50021 fp32 with a tail 66 us = 4.2 TB/s (three rows a compute unit, and a bit: the last ones are alone).  Small calls are bound by the
+// launch: 3840 rows of 18 actions take 10 us, 60 rows of 32768 9 us.  One pass over the row in memory costs a block's own latency (load, statistics,
+// barrier, gradient), which the other blocks of a compute unit cover; keeping the next row's loads in flight in the same block needed the registers of a
+// second row and was slower (spills).
 struct DistillArgs {
   const char* logits; int64_t ld;            // bytes from row to row
   char* grad; int64_t ldg;                   // null: loss only
@@ -399,6 +405,7 @@ template <int DT>
 void distill_dispatch(const DistillArgs& a, hipStream_t st) {
   const int nv = (a.V + Lg<DT>::VEC - 1) / Lg<DT>::VEC;
   if (nv <= 64 && a.K <= 64) distill_launch<DT, 64, 1>(a, st);
+  // (16384 rows, bf16, K 64, us: 1000 tokens 33 by a wave, 74 by 256 threads; 4000 tokens, K 64, 59 by two waves, 88 by 256 threads)
   else if (nv <= 256 && a.K <= 64) distill_launch<DT, 64, 4>(a, st);
   else if (nv <= 512 && a.K <= 128) distill_launch<DT, 128, 4>(a, st);
   else if (nv <= 10 * 256) distill_launch<DT, 256, 8>(a, st);
@@ -414,6 +421,9 @@ void distill_dispatch(const DistillArgs& a, hipStream_t st) {
 // K-th largest key of the buffer raises it, so that a row of n chunks appends about K (1 + log2 n) keys.  An element that only equals the bar comes
 // behind K others and is left out.  Should the buffer overflow all the same (rising rows), the lanes that found no room wait while it is cut to T keys,
 // and a chunk that alone would fill it is held to the exact K-th of its threads' maxima: K threads, EPT K keys, the room there is.
+// 3840 rows of 32768 bf16, K 32: 62 us = 4.1 TB/s, 1009 of 100003 fp16 at odd addresses, K 128: 64 us = 3.2 TB/s.  Long rows are bound by what an element
+// costs beside its load (maximum, exponential, comparison with the bar: 7 instructions); short ones with large K by the buffer: choosing the bar and
+// ordering K keys (each counts those above it, n^2 / 64 comparisons a block).  16384 rows of 1000: K 8 20 us, K 64 46, K 256 379.
 struct TopArgs {
   const char* logits; int64_t ld;
   int32_t* idx; float* val; float* lse;
@@ -694,6 +704,7 @@ __global__ __launch_bounds__(T) void top_join_kernel(TopArgs a) {
 }
 
 // A vocabulary of a few tokens (an action set): one token a lane, G lanes a row, 64 / G rows a wave; a token's place is the number of tokens before it.
+// 15360 rows of 18: 8 us, of which 1.6 MB are 0.4: the launch, then 18 shuffles.
 template <int DT, int G>
 __global__ __launch_bounds__(256) void top_small_kernel(TopArgs a) {
   const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -779,6 +790,9 @@ template <int DT> void top_dispatch(const TopArgs& a, const TopPlan& p, hipStrea
 //   verify_stats_kernel           (maximum, sum) in fp32 of the drafted positions' rows
 //   verify_sums_kernel<VF_STATS>  acceptance, and the fp64 sums of the one or two rows that the token is drawn from
 //   verify_pick_kernel<VF_STATS>  the rest as above
+// Bound: at 64 sequences of up to 8 drafts, 131072 bf16, 80 us: statistics 29 (220 MB at most, rows behind n_draft unread: exponentials and loads alike), sums 21
+// and pick 29 (17 and 34 MB: 20 fp64 instructions an exponential, at half rate, and the chain acceptance, chunk sums, last block, scan, token).  One sequence
+// of 4 drafts: sums 6, pick 15 (that chain alone).  37 sequences of 5 looked-up drafts, 50021 fp16: 13 and 15.  120 sequences of 7, 18 actions: one kernel, 8.
 constexpr int VF_T = 256, VF_WAVES = VF_T / 64, VF_CHUNK = 2048;   // 32 tokens a lane: what a chunk costs beside its exps (reductions) is shared by that many
 enum { VF_STATS, VF_SUMS, VF_ONE };          // three kernels, two, one
 struct VfSum { double e, s; };               // s 2^e; nothing: s = 0, e = -inf; a NaN among the logits: s NaN; +inf: e = +inf
