@@ -556,6 +556,38 @@ def test_captured_and_replayed(ctx):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("looked_up", [False, True])
+@pytest.mark.parametrize("B, K, V", [(120, 7, 18), (30, 3, 700), (4, 3, 9000), (64, 3, 50001), (6, 0, 5000)])
+def test_verify_captured_and_replayed(ctx, B, K, V, looked_up):
+    """Each form of the verification (one, two, three kernels) in a graph, replayed on new inputs with eager calls between."""
+    def inputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        t = 3 * torch.randn(B, K + 1, V, generator=g, device="cuda")
+        d = t[:, :K] + 0.4 * torch.randn(B, K, V, generator=g, device="cuda")
+        x = torch.randint(0, V, (B, K), generator=g, device="cuda", dtype=torch.int32)
+        if K and seed % 2:
+            x = d.argmax(-1).int()
+        return t, x, torch.rand(B, K, generator=g, device="cuda"), torch.rand(B, generator=g, device="cuda"), d, torch.randint(0, K + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+
+    def call(t, x, ua, us, d, n):
+        return TK.verify_drafts(ctx, t, x, ua, us, draft_logits=None if looked_up or not K else d, n_draft=n)
+    ins = inputs(1)
+    call(*ins)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call(*ins)
+    for seed in (2, 3, 4, 5):
+        new = inputs(seed)
+        eager = call(*new)
+        for a, b in zip(ins, new):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, eager):
+            assert torch.equal(a, b)
+
+
 def test_two_streams_at_once(ctx):
     ins = [step_inputs(10 + i) for i in range(2)]
     want = [[t.clone() for t in step(ctx, *i)] for i in ins]
