@@ -1074,14 +1074,17 @@ __device__ double vf_scan(double v, double* ss, double* total) {
   return v;
 }
 
-// What a token weighs in the draw: p, max(p - q, 0) where there is a draft row, or p but for one token
+// What a token weighs in the draw: p, max(p - q, 0) where there is a draft row, or p but for one token.  p and q are known to 2.7e-12 of themselves each
+// (VfExp's series, in the exponential and in the sum): what they differ by less than 2^-37 of is no difference.  Without that, of rows that are equal, or equal
+// up to a constant, p - q left roundings at half of the tokens, and the token was drawn from those instead of from p.  It goes into q's factor: no work.
+constexpr double VF_SAME = 0x1p-37;
 template <int DT> struct VfWeight {
   const char *prow, *qrow;
   VfExp ep, eq;
   double np, nq, none;
   int V, skip;
   __device__ __forceinline__ VfWeight(const VerifyArgs& a, const double* table, const char* prow, const VfSum& ps, const char* qrow, const VfSum& qs)
-    : prow(prow), qrow(qrow), ep{table, 32.0 * vf_slope(a, ps.e), 32.0 * ps.e}, eq{table, 32.0 * vf_slope(a, qs.e), 32.0 * qs.e}, np(1.0 / ps.s), nq(1.0 / qs.s),
+    : prow(prow), qrow(qrow), ep{table, 32.0 * vf_slope(a, ps.e), 32.0 * ps.e}, eq{table, 32.0 * vf_slope(a, qs.e), 32.0 * qs.e}, np(1.0 / ps.s), nq((1.0 + VF_SAME) / qs.s),
       none(2.0 * VF_NOTHING * np), V(a.V), skip(-1) {}
   __device__ __forceinline__ void leave_out(int token) { if ((uint32_t)token < (uint32_t)V) skip = token; }   // a looked-up token that was rejected
   __device__ __forceinline__ bool less() const { return qrow || skip >= 0; }

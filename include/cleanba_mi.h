@@ -319,7 +319,8 @@ int cbm_distill_loss_grad(cbm_ctx* ctx, const void* logits, int32_t dtype, int32
  *    elements (0 allowed: shared rows); draft_tokens i32 [batch][drafts]; n_draft i32 [batch] or NULL: how many of them count (clamped to [0, drafts];
  *    rows behind are not read); u_accept f32 [batch][drafts], u_sample f32 [batch] in [0, 1).
  *  Draft i is accepted while u_accept_i q_i(x_i) < p_i(x_i).  At the first rejection a one token is drawn from max(p_a - q_a, 0) (from p_a where that is 0
- *    everywhere), after n acceptances from p_n: the first token whose cumulative weight exceeds u_sample times the whole.
+ *    everywhere; where p_a and q_a agree to 2^-37 they are equal), after n acceptances from p_n: the first token whose cumulative weight exceeds u_sample
+ *    times the whole.
  *  tokens i32 [batch][drafts+1]: the accepted ones, the drawn one, then -1; accepted i32 [batch]; logprobs f32 [batch][drafts+1] or NULL: log p of each
  *    token, 0 behind the last.  temperature 0: p is one-hot at the largest logit (lowest index of equal ones), random numbers and draft_logits are not
  *    looked at and may be NULL, logprobs are 0.

@@ -1,0 +1,63 @@
+"""GPU tests of the token-policy operators where two answers lie next to each other: equal rows, borders between tokens, huge and poisoned logits.
+
+The 64-bit reference is tests/token_ref.py.  What a draw or an acceptance goes by is held to 64 bits: a probability's exponential is off by 1.33e-12 at most
+(a series to the fourth power on [-1/64, 1/64] in powers of two, an argument of up to 1000 rounded once), its row's sum by the same, so that a probability and a
+border between two tokens are off by at most 2.7e-12, and a log-probability by that and by its own rounding to fp32."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from cleanba_amd import tokens as TK
+from tests import token_ref as R
+from tests.test_gpu_tokens import D, DT, E, check_top, ctx, cuda, teacher  # noqa: F401  (ctx: the fixture)
+
+pytestmark = pytest.mark.gpu
+P64 = 2.7e-12   # a probability, relatively; a cumulative one
+
+
+def repeated(arrays, times):
+    return [torch.as_tensor(a).cuda().repeat(times, *[1] * (a.ndim - 1)) for a in arrays]
+
+
+def verify_many(ctx, times, p, x, ua, us, q, n=None, tau=1.0):
+    """The batch `times` over (a large call goes through other kernels), one copy's answers after all have been found the same."""
+    tp, tx, tua, tus = repeated((p, x, ua, us), times)
+    tq = None if q is None else repeated((q,), times)[0]
+    tn = None if n is None else repeated((n,), times)[0]
+    out = [t.view(times, len(x), *t.shape[1:]) for t in TK.verify_drafts(ctx, tp, tx, tua, tus, draft_logits=tq, n_draft=tn, temperature=tau)]
+    for t in out:
+        assert torch.equal(t, t[:1].expand_as(t))
+    return [t[0].cpu().numpy() for t in out]
+
+
+# ------------------------------------------------------------------------------------------ rejected with nothing left of p
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("V, times", [(30, 1), (9000, 1), (9000, 130)])   # one kernel, two, three
+def test_verify_draws_from_p_where_the_draft_equals_it(ctx, V, times, dtype):
+    """max(p - q, 0) is 0 everywhere where the rows are equal, or equal up to a constant: the token comes from p, not from what roundings leave of p - q.
+    Logits are multiples of 2^-8 below 16 (12 bits and a sign: exact in fp16 up to 8), so that the shifted rows are shifted exactly."""
+    rng = np.random.default_rng(V)
+    B, K, tau = 24, 2, 0.9
+    p = np.clip(np.round(rng.normal(0, 2, (B, K + 1, V)) * 64) / 64, -7, 7)
+    q = p[:, :K].copy()
+    x = rng.integers(0, V, (B, K)).astype(np.int32)
+    ua, us = rng.random((B, K), dtype=np.float32) * np.float32(0.9), rng.random(B, dtype=np.float32)
+    x[0:4, 0] = -1                             # outside the vocabulary: rejected
+    x[4:8, 0] = V
+    x[8:12, 0] = 7                             # masked in both rows: 0 < 0 is not
+    p[8:12, 0, 7] = q[8:12, 0, 7] = -math.inf
+    q[12:16] += np.array([1.0, -3.0, 0.25, 7.0])[:, None, None]   # equal up to a constant
+    x[12:16, 0] = -1
+    x[16:20, 1] = -1                           # the second draft (the first is accepted: u q < p)
+    q[20:24, 0, 5] = -math.inf                 # but one token: it alone is left
+    p[20:24, 0, 5] = -7.0
+    x[20:24, 0] = -1
+    p, q = (a.astype(np.float32 if dtype == "f32" else np.float16) for a in (p, q))
+    tok, acc, lp = verify_many(ctx, times, p, x, ua, us, q, tau=tau)
+    for b in range(B):
+        want, a, logs, margin = R.verify(p[b].astype(np.float64), q[b].astype(np.float64), x[b], K, ua[b], us[b], tau)
+        assert margin > 1e-5, (b, margin)      # (of the draw: a million times its distance from a border)
+        assert tok[b].tolist() == want and acc[b] == a, (b, tok[b], want)
+        assert np.all(np.abs(lp[b] - np.array(logs)) <= D(V) + 2 * E * np.abs(logs)), (b, lp[b], logs)
