@@ -779,7 +779,7 @@ template <int DT> void top_dispatch(const TopArgs& a, const TopPlan& p, hipStrea
 // The drawn token lies between two neighbours of a cumulative sum over the whole vocabulary: sums that are off by 1e-7 would move one token in a few
 // hundred, so that the row it is drawn from is summed in fp64, exponentials too.  They are 2^(z C - E), C = log2(e) / tau, with a whole number E a chunk of
 // 2048 tokens (the maximum's exponent, rounded up): sums of different chunks are brought together by exact shifts of the exponent.  An acceptance compares
-// two numbers, and sums of fp32 exponentials do for it.
+// two numbers, and sums of fp32 exponentials do for it where the two are not next to each other (vf_accept).
 // Rows of one chunk and few drafts, one kernel:
 //   verify_one_kernel             a block a sequence: its rows' sums, then all that follows
 // Small calls, two kernels (launches are what they cost):
@@ -810,6 +810,7 @@ struct VerifyArgs {
   int B, K, V, nchunk, nstat, nsplit, npick; // splits of a row in fp32 and in fp64, blocks a sequence in the last kernel
   float c;
   double C, C2;                              // log2(e) / tau, and the power of two not below it
+  double close;                              // VF_STATS: how near, relatively, u q and p may be for fp32 sums to tell which is less
 };
 __device__ __forceinline__ int vf_drafts(const VerifyArgs& a, int b) {
   const int n = a.n_draft ? a.n_draft[b] : a.K;
@@ -903,68 +904,6 @@ __global__ __launch_bounds__(VF_T) void verify_stats_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) a.stats[blockIdx.x] = ms;
 }
 
-// How many drafts of sequence b are accepted; every thread of the block gets it.  srow: the rows' sums, target 0 .. n, draft 0 .. n - 1 behind them
-// (from fp32 statistics target 0 .. n - 1; VF_ONE: the caller has filled them in).  `write`: the block that writes what is known then.
-template <int DT, int HOW> __device__ int vf_accept(const VerifyArgs& a, int b, int n, bool write, const double* table, VfSum* srow, int* sat) {
-  const int tid = threadIdx.x;
-  const int64_t k0 = (int64_t)b * a.K, t0 = (int64_t)b * (a.K + 1);
-  int x = -1;
-  float u = 0.0f, zp = 0.0f, zq = 0.0f;
-  if (tid < n) {
-    x = a.tokens[k0 + tid];
-    u = a.u_accept[k0 + tid];
-    if ((uint32_t)x < (uint32_t)a.V) {
-      zp = tk_at<DT>(a.target + b * a.tb + tid * a.tp, x);
-      if (a.draft) zq = tk_at<DT>(a.draft + b * a.db + tid * a.dp, x);
-    }
-  }
-  if (tid == 0) *sat = n;
-  const int heads = HOW == VF_STATS ? n : n + 1, rows = HOW == VF_ONE ? 0 : heads + (a.draft ? n : 0);
-  for (int r = tid >> 4; r < rows; r += VF_T / 16) {   // 16 lanes a row
-    VfSum s = {-INFINITY, 0.0};
-    if constexpr (HOW == VF_SUMS) {
-      const VfSum* p = a.parts + (r < heads ? t0 + r : (int64_t)a.B * (a.K + 1) + k0 + r - heads) * a.nsplit;
-      for (int i = tid & 15; i < a.nsplit; i += 16) s = vf_add(s, p[i]);
-      for (int o = 8; o > 0; o >>= 1) s = vf_add(s, VfSum{__shfl_xor(s.e, o, 16), __shfl_xor(s.s, o, 16)});
-    } else {
-      const MS* p = a.stats + (r < heads ? k0 + r : (int64_t)a.B * a.K + k0 + r - heads) * a.nstat;
-      float m = -INFINITY;
-      for (int i = tid & 15; i < a.nstat; i += 16) m = fmaxf(m, p[i].m);
-      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
-      for (int i = tid & 15; i < a.nstat; i += 16) s.s += p[i].s * (double)tk_exp2((p[i].m - tk_base(m)) * a.c);
-      for (int o = 8; o > 0; o >>= 1) s.s += __shfl_xor(s.s, o, 16);
-      s.e = m == -INFINITY ? m : vf_ceil(a, m);
-      if ((tid & 15) == 0) s.s *= exp2(fma((double)m, vf_slope(a, s.e), -s.e));   // (the sum was relative to m)
-    }
-    if ((tid & 15) == 0) srow[r] = s;
-  }
-  __syncthreads();
-  double logp = 0.0;
-  if (tid < n) {
-    bool ok = false;
-    if ((uint32_t)x < (uint32_t)a.V && vf_good(srow[tid])) {
-      const VfSum ps = srow[tid];
-      const double p = vf_prob(table, a, ps, zp);
-      double q = 1.0;
-      if (a.draft) {
-        const VfSum qs = srow[heads + tid];
-        q = vf_good(qs) ? vf_prob(table, a, qs, zq) : NAN;
-      }
-      ok = (double)u * q < p;                // (a NaN: not accepted)
-      if (ok && write) logp = vf_logp(a, ps, zp);
-    }
-    if (!ok) atomicMin(sat, tid);
-  }
-  __syncthreads();
-  const int at = *sat;
-  if (write) {
-    if (tid < at) { a.out[t0 + tid] = x; if (a.logprobs) a.logprobs[t0 + tid] = (float)logp; }
-    else if (tid > at && tid <= a.K) { a.out[t0 + tid] = -1; if (a.logprobs) a.logprobs[t0 + tid] = 0.0f; }
-    if (tid == 0) a.accepted[b] = at;
-  }
-  return at;
-}
-
 // a chunk's vectors of a lane
 template <int DT> __device__ __forceinline__ void vf_chunk(Pack (&y)[VF_CHUNK / 64 / Lg<DT>::VEC], const char* row, int ch, int V) {
   constexpr int U = VF_CHUNK / 64 / Lg<DT>::VEC;
@@ -1006,6 +945,103 @@ template <int DT> __device__ __forceinline__ VfSum vf_sum_chunk(Pack (&x)[VF_CHU
   return VfSum{m == -INFINITY ? -INFINITY : E, s};
 }
 
+// the fp64 sum of a whole row, by the block's waves; every thread gets it.  `part` holds one a wave
+template <int DT> __device__ VfSum vf_sum_row(const VerifyArgs& a, const char* row, const double* table, VfSum* part) {
+  constexpr int U = VF_CHUNK / 64 / Lg<DT>::VEC;
+  const int wave = threadIdx.x >> 6;
+  VfSum all = {-INFINITY, 0.0};
+  for (int ch = wave; ch < a.nchunk; ch += VF_WAVES) {
+    Pack x[U];
+    vf_chunk<DT>(x, row, ch, a.V);
+    all = vf_add(all, vf_sum_chunk<DT>(x, ch, a, table));
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[wave] = all;
+  __syncthreads();
+  all = part[0];
+#pragma unroll
+  for (int w = 1; w < VF_WAVES; ++w) all = vf_add(all, part[w]);
+  return all;
+}
+
+// How many drafts of sequence b are accepted; every thread of the block gets it.  srow: the rows' sums, target 0 .. n, draft 0 .. n - 1 behind them
+// (from fp32 statistics target 0 .. n - 1; VF_ONE: the caller has filled them in).  `write`: the block that writes what is known then.
+// From fp32 statistics a draft whose two sides lie nearer to each other than those can tell (a.close) is decided by fp64 sums of its rows, which each block of the
+// sequence forms for itself: a few drafts in 10^5.  So a decision does not go by how many others are in the call.
+enum : uint8_t { VF_NO, VF_YES, VF_CLOSE };
+template <int DT, int HOW> __device__ int vf_accept(const VerifyArgs& a, int b, int n, bool write, const double* table, VfSum* srow, int* sat, uint8_t* sstate = nullptr,
+                                                    VfSum* spart = nullptr) {   // (the last two: VF_STATS)
+  const int tid = threadIdx.x;
+  const int64_t k0 = (int64_t)b * a.K, t0 = (int64_t)b * (a.K + 1);
+  int x = -1;
+  float u = 0.0f, zp = 0.0f, zq = 0.0f;
+  if (tid < n) {
+    x = a.tokens[k0 + tid];
+    u = a.u_accept[k0 + tid];
+    if ((uint32_t)x < (uint32_t)a.V) {
+      zp = tk_at<DT>(a.target + b * a.tb + tid * a.tp, x);
+      if (a.draft) zq = tk_at<DT>(a.draft + b * a.db + tid * a.dp, x);
+    }
+  }
+  if (tid == 0) *sat = n;
+  const int heads = HOW == VF_STATS ? n : n + 1, rows = HOW == VF_ONE ? 0 : heads + (a.draft ? n : 0);
+  for (int r = tid >> 4; r < rows; r += VF_T / 16) {   // 16 lanes a row
+    VfSum s = {-INFINITY, 0.0};
+    if constexpr (HOW == VF_SUMS) {
+      const VfSum* p = a.parts + (r < heads ? t0 + r : (int64_t)a.B * (a.K + 1) + k0 + r - heads) * a.nsplit;
+      for (int i = tid & 15; i < a.nsplit; i += 16) s = vf_add(s, p[i]);
+      for (int o = 8; o > 0; o >>= 1) s = vf_add(s, VfSum{__shfl_xor(s.e, o, 16), __shfl_xor(s.s, o, 16)});
+    } else {
+      const MS* p = a.stats + (r < heads ? k0 + r : (int64_t)a.B * a.K + k0 + r - heads) * a.nstat;
+      float m = -INFINITY;
+      for (int i = tid & 15; i < a.nstat; i += 16) m = fmaxf(m, p[i].m);
+      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
+      for (int i = tid & 15; i < a.nstat; i += 16) s.s += p[i].s * (double)tk_exp2((p[i].m - tk_base(m)) * a.c);
+      for (int o = 8; o > 0; o >>= 1) s.s += __shfl_xor(s.s, o, 16);
+      s.e = m == -INFINITY ? m : vf_ceil(a, m);
+      if ((tid & 15) == 0) s.s *= exp2(fma((double)m, vf_slope(a, s.e), -s.e));   // (the sum was relative to m)
+    }
+    if ((tid & 15) == 0) srow[r] = s;
+  }
+  __syncthreads();
+  const auto decide = [&](const VfSum& ps, const VfSum& qs, double* p, double* uq) {   // thread `tid`'s draft; a row that is no distribution: not accepted
+    if ((uint32_t)x >= (uint32_t)a.V || !vf_good(ps) || (a.draft && !vf_good(qs))) return false;
+    *p = vf_prob(table, a, ps, zp);
+    *uq = (double)u * (a.draft ? vf_prob(table, a, qs, zq) : 1.0);
+    return *uq < *p;                         // (a NaN: not accepted)
+  };
+  double logp = 0.0;
+  if (tid < n) {
+    double p = 0.0, uq = 0.0;
+    const bool ok = decide(srow[tid], a.draft ? srow[heads + tid] : srow[tid], &p, &uq);
+    if constexpr (HOW == VF_STATS) sstate[tid] = fabs(uq - p) < a.close * fmax(uq, p) ? VF_CLOSE : (ok ? VF_YES : VF_NO);
+    if (!ok || (HOW == VF_STATS && sstate[tid] == VF_CLOSE)) atomicMin(sat, tid);
+    else if (write) logp = vf_logp(a, srow[tid], zp);
+  }
+  __syncthreads();
+  int at = *sat;
+  if constexpr (HOW == VF_STATS) {
+    while (at < n && sstate[at] == VF_CLOSE) {   // (the same for every thread)
+      const VfSum ps = vf_sum_row<DT>(a, a.target + b * a.tb + at * a.tp, table, spart);
+      const VfSum qs = a.draft ? vf_sum_row<DT>(a, a.draft + b * a.db + at * a.dp, table, spart) : ps;
+      if (tid == at) {
+        double p, uq;
+        sstate[at] = decide(ps, qs, &p, &uq) ? VF_YES : VF_NO;
+        logp = vf_logp(a, ps, zp);
+      }
+      __syncthreads();
+      while (at < n && sstate[at] == VF_YES) ++at;
+      __syncthreads();
+    }
+  }
+  if (write) {
+    if (tid < at) { a.out[t0 + tid] = x; if (a.logprobs) a.logprobs[t0 + tid] = (float)logp; }
+    else if (tid > at && tid <= a.K) { a.out[t0 + tid] = -1; if (a.logprobs) a.logprobs[t0 + tid] = 0.0f; }
+    if (tid == 0) a.accepted[b] = at;
+  }
+  return at;
+}
+
 template <int DT, int HOW>
 __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
   constexpr int U = VF_CHUNK / 64 / Lg<DT>::VEC;
@@ -1031,9 +1067,10 @@ __global__ __launch_bounds__(VF_T) void verify_sums_kernel(VerifyArgs a) {
   } else {
     __shared__ VfSum srow[2 * TK_MAX_DRAFTS];
     __shared__ int sat;
+    __shared__ uint8_t sstate[TK_MAX_DRAFTS];
     const bool of_draft = row >= a.B;
     const int b = (int)(of_draft ? row - a.B : row), n = vf_drafts(a, b);
-    const int at = vf_accept<DT, VF_STATS>(a, b, n, !of_draft && split == 0, table, srow, &sat);
+    const int at = vf_accept<DT, VF_STATS>(a, b, n, !of_draft && split == 0, table, srow, &sat, sstate, part);
     if (!of_draft && split == 0 && tid == 0) a.done[b] = 0;
     if (of_draft && at >= n) return;
     z = of_draft ? a.draft + b * a.db + at * a.dp : a.target + b * a.tb + at * a.tp;
@@ -1563,6 +1600,10 @@ extern "C" int cbm_verify_drafts(cbm_ctx* c, const void* target_logits, int32_t 
   char* ws = (char*)workspace;
   a.sums = (VfSum*)ws; a.parts = (VfSum*)(ws + p.o_parts); a.rest = (double*)(ws + p.o_rest); a.stats = (MS*)(ws + p.o_stats); a.done = (uint32_t*)(ws + p.o_done);
   a.B = batch; a.K = drafts; a.V = vocab; a.nsplit = p.nsplit; a.nchunk = p.nchunk; a.nstat = p.nstat; a.npick = p.npick;
+  // A sum in fp32 (verify_stats_kernel) is off by, in units of 2^-24: three roundings of an argument, weighted by the probabilities (3 log2 V <= 57), the exponential
+  // and the join (12), the terms of a step (32), four a step (rescaling, adding).  p and q have one each.
+  const int64_t step = VF_T * 32, steps = p.nstat ? ((vocab + p.nstat - 1) / p.nstat + 8 + step - 1) / step : 0;   // (a split's end is rounded to a vector)
+  a.close = 2.0 * (57 + 12 + 32 + 4 * (double)steps) * 0x1p-24;
   a.C = greedy ? 0.0 : TK_LOG2E / temperature; a.C2 = greedy ? 0.0 : std::exp2(std::ceil(std::log2(a.C))); a.c = (float)a.C;
   hipStream_t st = tk_stream(c, stream);
   if (dtype == CBM_F32) verify_dispatch<CBM_F32>(a, p, greedy, st);
