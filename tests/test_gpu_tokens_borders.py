@@ -94,3 +94,16 @@ def test_verify_accepts_by_64_bits_whatever_the_batch(ctx, looked_up):
     few = [verify_many(ctx, 1, *(a[i:i + 7] for a in (p, x, ua, us)), None if looked_up else q[i:i + 7], tau=tau) for i in range(0, 70, 7)]
     for k in range(2):
         assert np.array_equal(np.concatenate([f[k] for f in few]), got[k][:70])
+
+
+# ------------------------------------------------------------------------------------------ log-probabilities
+@pytest.mark.parametrize("V, times", [(30, 1), (9000, 1), (9000, 500)])
+def test_verify_log_probabilities_of_huge_logits(ctx, V, times):
+    """Equal logits of 1e7 to 4.5e10: the token's exponent z log2(e) / tau and the row's are alike, their difference is exact."""
+    z = np.float32([1e7, -3e7, 1.234567e9, 7.7777e9, -2.3456e10, 3.21e10, 4.1e10, 4.4321e10])
+    p = np.repeat(z[:, None], V, 1)[:, None, :]
+    B = len(z)
+    live = 17
+    p[:, 0, live:] = -math.inf
+    _, _, lp = verify_many(ctx, times, p, np.zeros((B, 0), np.int32), np.zeros((B, 0), np.float32), np.full(B, 0.5, np.float32), None)
+    assert np.abs(lp[:, 0] + math.log(live)).max() <= E * math.log(live) + 1e-10, lp[:, 0] + math.log(live)
