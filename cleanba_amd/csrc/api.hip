@@ -11,9 +11,12 @@
 //     `u` reads version max(0,u-2) with --concurrency (the `update != 2` skew, ppo:287-304) or
 //     u-1 without.
 #include "cbm_ctx.h"
+#include <errno.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
+#include <sys/mman.h>
+#include <unistd.h>
 #include <string>
 #include <mutex>
 #include <condition_variable>
@@ -513,17 +516,32 @@ extern "C" int cbm_actor_step_async(cbm_ctx* c, int32_t s, const uint8_t* obs, c
   sl.t += 1;
   return 0;
 }
+// whether every page of [p, p + n) is mapped: a wrong pointer or length is told from a system that page-locks no existing memory (HIP gives one error for both)
+static bool host_mapped(const void* p, size_t n) {
+  const uintptr_t page = (uintptr_t)sysconf(_SC_PAGESIZE), end = (uintptr_t)p + n;
+  if (end < (uintptr_t)p) return false;
+  unsigned char in[1024];
+  for (uintptr_t at = (uintptr_t)p & ~(page - 1); at < end;) {
+    const uintptr_t left = end - at, len = left < page * sizeof(in) ? left : page * sizeof(in);
+    if (mincore((void*)at, len, in) != 0 && errno == ENOMEM) return false;
+    at += len;
+  }
+  return true;
+}
 extern "C" int cbm_host_register(cbm_ctx* c, void* ptr, int64_t nbytes) {
-  CBM_HIP(hipSetDevice(c->cfg.device));
   if (!ptr || nbytes <= 0) { cbm_set_error("cbm_host_register: empty buffer"); return -1; }
+  if (!host_mapped(ptr, (size_t)nbytes)) { cbm_set_error("cbm_host_register: %p + %lld is not mapped memory of this process", ptr, (long long)nbytes); return -1; }
+  if (!c) { cbm_set_error("cbm_host_register: null context"); return -1; }
+  CBM_HIP(hipSetDevice(c->cfg.device));
   const hipError_t e = hipHostRegister(ptr, (size_t)nbytes, hipHostRegisterDefault);
+  std::lock_guard<std::mutex> lk(c->pageable_mu);
   if (e == hipErrorInvalidValue || e == hipErrorNotSupported) {   // a system that page-locks no existing memory: staged copies, same results
     (void)hipGetLastError();                 // (or the next call's check reports it)
-    std::lock_guard<std::mutex> lk(c->pageable_mu);
     c->pageable.insert(ptr);
-    return 0;
+    return CBM_HOST_PAGEABLE;
   }
   CBM_HIP(e);
+  c->pageable.erase(ptr);                    // (another buffer was refused at this address before)
   return 0;
 }
 extern "C" int cbm_host_unregister(cbm_ctx* c, void* ptr) {

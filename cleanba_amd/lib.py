@@ -15,6 +15,7 @@ SO_PATH = os.environ.get("CBM_SO", os.path.join(_HERE, "libcleanba_mi.so"))  # C
 NET_NATURE, NET_IMPALA_RESNET = 0, 1
 ALGO_PPO, ALGO_IMPALA = 0, 1
 F32, BF16, F16 = 0, 1, 2              # CBM_F32 ..: types of token logits
+HOST_PAGEABLE = 1                     # CBM_HOST_PAGEABLE
 LEARNER_STREAM = 2 ** (8 * C.sizeof(C.c_void_p)) - 1   # CBM_LEARNER_STREAM
 FRAME = 4 * 84 * 84
 
@@ -309,9 +310,12 @@ class Context:
         _chk(self.lib.cbm_actor_record_host(self.h, int(slot), r.ctypes.data))
 
     def host_register(self, arr):
-        """Page-locks a numpy array the env reuses for its observations (cbm_host_register)."""
+        """Page-locks a numpy array the env reuses for its observations (cbm_host_register); False where the system refused and it stays pageable."""
         assert arr.flags["C_CONTIGUOUS"]
-        _chk(self.lib.cbm_host_register(self.h, _p(arr), C.c_int64(arr.nbytes)))
+        rc = self.lib.cbm_host_register(self.h, _p(arr), C.c_int64(arr.nbytes))
+        if rc != HOST_PAGEABLE:
+            _chk(rc)
+        return rc == 0
 
     def host_unregister(self, arr):
         _chk(self.lib.cbm_host_unregister(self.h, _p(arr)))

@@ -210,10 +210,10 @@ def _rollout(key, args, algo, engine, writer, slot, world_size, process_index, s
         n = seen.get(ptr, 0) + 1
         if n >= 2 and len(pinned) < MAX_PINNED and obs.flags.c_contiguous:
             try:
-                register(obs)
-                pinned[ptr] = obs          # keeps the array alive while it is registered
+                locked = register(obs) is not False
             except RuntimeError:
-                pinned[ptr] = None         # not registrable (e.g. a read-only mapping): do not retry every step
+                locked = False
+            pinned[ptr] = obs if locked else None   # keeps the array alive while it is registered; None: stays pageable, not tried again every step
             seen.pop(ptr, None)
             return
         if len(seen) > 64:                 # fresh arrays every step: forget the oldest addresses

@@ -133,7 +133,9 @@ int cbm_actor_record_host(cbm_ctx* ctx, int32_t slot, const float* reward);
 /* Page-lock a host buffer the env hands to cbm_actor_step_host / cbm_actor_commit again and again (envpool's recv buffers, a numpy array
  * the host reuses): the 3.39 MB observation upload of a 120-env step (the jnp transfer inside get_action_and_value, ppo:313) then goes by
  * DMA from the caller's pages instead of through the runtime's pageable staging.  Optional; unregister before freeing the memory.
- * Where the system refuses to page-lock memory that exists already the buffer stays pageable: 0 is returned, uploads are staged, results the same. */
+ * Where the system refuses to page-lock memory that exists already the buffer stays pageable: CBM_HOST_PAGEABLE is returned, uploads are staged,
+ * results the same, and it need not be unregistered.  A range that is not mapped memory is an error. */
+#define CBM_HOST_PAGEABLE 1
 int cbm_host_register(cbm_ctx* ctx, void* ptr, int64_t nbytes);
 int cbm_host_unregister(cbm_ctx* ctx, void* ptr);
 /* Device-env rollout: the built-in synthetic Atari-shaped env (cbm_synth_*) steps on the GPU, so

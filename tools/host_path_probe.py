@@ -54,9 +54,9 @@ ctx2 = L.Context(cfg)
 ctx2.set_params(init_nature_params(18, [0, 1], [0, 2], [0, 3]))
 ctx2.actor_set_key(0, np.array([0, 1], np.uint32))
 t0 = time.perf_counter()
-ctx2.host_register(obs)
-print("hipHostRegister    : %7.1f us (once)" % ((time.perf_counter() - t0) * 1e6))
-print("step_host pinned   : %7.1f us" % steps(ctx2, obs))
+locked = ctx2.host_register(obs)
+print("hipHostRegister    : %7.1f us (once)%s" % ((time.perf_counter() - t0) * 1e6, "" if locked else " REFUSED: the buffer stays pageable"))
+print("step_host %s : %7.1f us" % ("pinned  " if locked else "pageable", steps(ctx2, obs)))
 ctx2.host_unregister(obs)
 import os
 print("cpu %d  affinity %d cpus" % (os.sched_getcpu() if hasattr(os, "sched_getcpu") else -1, len(os.sched_getaffinity(0))))
