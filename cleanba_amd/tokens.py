@@ -37,10 +37,18 @@ def _logits(dev, t, name, dims=None):
     shape, strides = t.shape, t.stride()
     if not shape or (dims is not None and len(shape) != dims):
         raise ValueError(f"{name}: {dims or 'one or more'} dimensions are expected, got {tuple(shape)}")
+    if t.numel() > 0x7fffffff:
+        _fits(shape[-1], f"{name}: tokens")
+        _fits(shape[:-1].numel(), f"{name}: rows")
     if strides[-1] != 1 and shape[-1] > 1 and t.numel():
         raise ValueError(f"{name}: the vocabulary (the last axis) has to be dense, its stride is {strides[-1]}")
     _placed(dev, t, name)
     return _DTYPE[t.dtype], shape, strides
+
+
+def _fits(n, name):
+    if not -0x80000000 <= n <= 0x7fffffff:   # (the C calls take 32 bits, and ctypes cuts to them without a word)
+        raise ValueError(f"{name}: {n} is more than any call takes")
 
 
 def _placed(dev, t, name):
@@ -94,6 +102,7 @@ def top_logits(ctx, logits, k, temperature=1.0):
     """The k largest logits of each row of `logits` [..., vocab], falling, equal ones by rising index -> (idx int32 [..., k], values float32 [..., k],
     lse float32 [...] = log sum exp(logits / temperature)).  Slots beyond the logits above -inf hold -1 and -inf (cbm_top_logits)."""
     index, k = ctx.cfg.device, int(k)
+    _fits(k, "k")
     dtype, shape, strides = _logits(index, logits, "logits")
     rows, stride = _rows(logits, shape, strides, "logits")
     vocab, lead, dev = shape[-1], shape[:-1], logits.device
@@ -121,6 +130,7 @@ def distill_loss_grad(ctx, logits, teacher_idx, teacher_logits, teacher_lse=None
     if not isinstance(teacher_idx, torch.Tensor) or teacher_idx.dim() != len(shape):
         raise ValueError(f"teacher_idx: an int32 tensor of shape {tuple(lead) + ('k',)} is expected")
     k = teacher_idx.shape[-1]
+    _fits(k, "teacher_idx: slots")
     slots = lead + (k,)
     teacher_idx = _operand(index, teacher_idx, "teacher_idx", _i32, slots)
     teacher_logits = _operand(index, teacher_logits, "teacher_logits", _f32, slots)
