@@ -121,8 +121,8 @@ def distill_loss_grad(ctx, logits, teacher_idx, teacher_logits, teacher_lse=None
     """Distillation of the student's `logits` [..., vocab] from a teacher's top logits (idx int32, float32 [..., k]) -> (loss float32 [...], dlogits or None).
 
     teacher_lse float32 [...] keeps the teacher's mass outside its slots as one more class; without it the teacher is a softmax over the slots.
-    row_weight float32 [...] scales a row's loss and gradient; rows of weight 0 are not read.  in_place=True writes the gradient over the logits.
-    (cbm_distill_loss_grad)"""
+    row_weight float32 [...] scales a row's loss and gradient; rows of weight 0 are not read.  in_place=True writes the gradient over the logits
+    (their version counter rises).  Neither output has a graph: `logits.backward(dlogits)` takes a student further.  (cbm_distill_loss_grad)"""
     index = ctx.cfg.device
     dtype, shape, strides = _logits(index, logits, "logits")
     rows, stride = _rows(logits, shape, strides, "logits")
@@ -145,6 +145,8 @@ def distill_loss_grad(ctx, logits, teacher_idx, teacher_logits, teacher_lse=None
     if ctx.lib.cbm_distill_loss_grad(ctx.h, logits.data_ptr(), dtype, rows, vocab, stride, teacher_idx.data_ptr(), teacher_logits.data_ptr(), k,
                                      _ptr(teacher_lse), _ptr(row_weight), temperature, loss.data_ptr(), _ptr(grad), gstride, _raw_stream(index)):
         L._chk(-1)
+    if grad is logits:
+        torch.autograd.graph.increment_version(logits)   # as torch's own in-place operators: a backward that saved the logits notices
     return loss, grad
 
 

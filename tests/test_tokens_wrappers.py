@@ -38,3 +38,16 @@ def test_sizes_beyond_32_bits_are_refused(ctx):
         with pytest.raises(ValueError, match="more than any call takes"):
             call()
     assert not ctx.calls
+
+
+def test_in_place_is_seen_by_autograd(ctx):
+    """A backward that saved the logits must not take the gradient for them."""
+    idx, val = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2)
+    w = torch.ones(3, 5, requires_grad=True)
+    z = w.exp()                                # saves its result
+    TK.distill_loss_grad(ctx, z, idx, val)
+    z.sum().backward(retain_graph=True)        # out of place: nothing has changed
+    _, grad = TK.distill_loss_grad(ctx, z, idx, val, in_place=True)
+    assert grad is z
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
