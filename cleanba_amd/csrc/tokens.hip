@@ -442,6 +442,7 @@ __device__ __forceinline__ uint64_t top_key(float v, int e) { return ((uint64_t)
 __device__ __forceinline__ int top_index(uint64_t key) { return TK_MAX_VOCAB - 1 - (int)(key & (TK_MAX_VOCAB - 1)); }
 __device__ __forceinline__ uint32_t top_order_of(uint64_t key) { return (uint32_t)(key >> 19); }
 constexpr int TOP_KEY_BITS = 51;
+constexpr int TOP_SPLIT_T = 256;             // the threads of a block where rows are split (top_plan)
 
 // the largest bound that K of the block's T numbers (0: none) reach, or 0 where fewer are there; the first wave's work.  With slack, any bound that K .. K + slack
 // of them reach: a third of the steps.
@@ -675,7 +676,7 @@ __global__ __launch_bounds__(T) void top_kernel(TopArgs a) {
     fill = top_cut<T, MOST>(buf, fill, K, T, &bar, sh);
   }
   const MS ms = block_lse<T>(m, s, a.c, red);
-  if (a.nsplit > 1) {
+  if (T == TOP_SPLIT_T && a.nsplit > 1) {
     top_write<T>(buf, fill, K, nullptr, nullptr, a.ws_keys + (r * a.nsplit + split) * K);
     if (tid == 0) a.ws_ms[r * a.nsplit + split] = ms;
   } else {
@@ -739,7 +740,7 @@ TopPlan top_plan(int rows, int V, int K) {
   // Few rows leave compute units empty: up to 128 long ones are split until there are about 512 blocks, and joined (a second kernel); up to 255 others go to
   // wider blocks.  us split / not: 60 x 32768 bf16, K = 32, 20 / 15; 1 x 131072 bf16, K = 64, 21 / 30; 60 of them 21 / 31, 200 34 / 34; 1 x 100003 fp16, K = 128, 27 / 31,
   // 200 39 / 36; K = 256 (by 512 threads either way) 1 x 131072 38 / 40, 60 58 / 40.
-  const bool split = rows <= 128 && V > 49152 && K <= 128;
+  const bool split = rows <= 128 && V > 49152 && p.threads == TOP_SPLIT_T;   // (K <= 128)
   if (!split && rows < 256 && V > 16384) p.threads = 512;
   p.cap = top_ept(p.threads, V) * K + p.threads;
   if (split) {
@@ -755,7 +756,7 @@ template <int DT, int T, int EPT, int G, int KMAX> void top_launch(const TopArgs
   static_assert(2 * KMAX <= T, "or top_cut does not end");
   constexpr int MOST = EPT * KMAX / T + 1;   // cap <= MOST T
   hipLaunchKernelGGL((top_kernel<DT, T, EPT, G, MOST>), dim3((uint32_t)a.rows * p.nsplit), dim3(T), p.lds, st, a);
-  if (p.nsplit > 1) hipLaunchKernelGGL((top_join_kernel<T, MOST>), dim3(a.rows), dim3(T), p.lds, st, a);
+  if constexpr (T == TOP_SPLIT_T) if (p.nsplit > 1) hipLaunchKernelGGL((top_join_kernel<T, MOST>), dim3(a.rows), dim3(T), p.lds, st, a);
 }
 template <int DT, int G> void top_launch_small(const TopArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((top_small_kernel<DT, G>), dim3((uint32_t)(((int64_t)a.rows * G + 255) / 256)), dim3(256), 0, st, a);
