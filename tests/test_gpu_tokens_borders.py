@@ -107,3 +107,118 @@ def test_verify_log_probabilities_of_huge_logits(ctx, V, times):
     p[:, 0, live:] = -math.inf
     _, _, lp = verify_many(ctx, times, p, np.zeros((B, 0), np.int32), np.zeros((B, 0), np.float32), np.full(B, 0.5, np.float32), None)
     assert np.abs(lp[:, 0] + math.log(live)).max() <= E * math.log(live) + 1e-10, lp[:, 0] + math.log(live)
+
+
+# ------------------------------------------------------------------------------------------ draws next to their border
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V, B", [(300, 96), (50021, 48), (131072, 16)])
+def test_verify_draws_next_to_a_border(ctx, V, B, dtype):
+    """u_sample on the floats next to a cumulative probability, on either side: sums in fp32 would move many of these tokens.  Log-probabilities to fp32's
+    own rounding."""
+    rng = np.random.default_rng(V + 1)
+    t = torch.as_tensor(rng.normal(0, 2, (B, 1, V)), dtype=torch.float32).to(DT[dtype])
+    p = t.double().numpy()
+    us, want, logs = np.zeros(B, np.float32), [], []
+    for b in range(B):
+        d = R._dist(p[b, 0], 1.0)
+        c = np.cumsum(d) / d.sum()
+        while True:
+            j = int(rng.choice(np.flatnonzero((d[:-1] > 3e-7) & (d[1:] > 3e-7) & (c[:-1] < 0.999))))
+            near = np.float32(c[j])
+            below = near if float(near) < c[j] else np.nextafter(near, np.float32(0))
+            u = below if b % 2 else np.nextafter(below, np.float32(2))
+            if abs(float(u) - c[j]) > 1e-11:   # (the border itself is summed here to 1e-14)
+                break
+        us[b] = u
+        want.append(j if b % 2 else j + 1)
+        logs.append(math.log(d[want[-1]]))
+    tok, _, lp = (x.cpu().numpy() for x in TK.verify_drafts(ctx, t.cuda(), None, None, cuda(us)))
+    assert tok[:, 0].tolist() == want
+    assert np.all(np.abs(lp[:, 0] - logs) <= 1.001 * E * np.abs(logs) + 1e-10)
+
+
+# ------------------------------------------------------------------------------------------ NaN and infinities
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V, k", [(18, 4), (60, 64), (1000, 16), (3000, 200), (60000, 32)])   # a token a lane, one block a row (64 and 512 threads), split rows
+def test_top_logits_poisoned_rows(ctx, V, k, dtype):
+    """NaN is never taken and makes the log-sum-exp NaN, +inf is taken first and makes it +inf, at any place of a row; rows beside them do not notice."""
+    rng = np.random.default_rng(V)
+    z = rng.normal(0, 2, (12, V))
+    z[1, 0] = z[2, V - 1] = z[3, V // 2] = z[4, ::2] = math.nan
+    z[5, 1] = z[6, V - 1] = math.inf
+    z[7] = math.nan
+    z[8] = -math.inf
+    z[9, 1:] = -math.inf
+    z[10, :V - 1] = math.nan
+    z[11, 3], z[11, 7] = math.inf, -math.inf
+    t = torch.as_tensor(z, dtype=torch.float32).to(DT[dtype])
+    check_top(ctx, t.double().numpy(), t.cuda(), k)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [40, 5001, 70001])
+def test_distill_poisoned_rows(ctx, V, dtype, tail):
+    """A NaN or +inf in a row, at a token of the teacher or at another, makes that row's loss and gradient NaN, and no other's."""
+    rng = np.random.default_rng(V)
+    z = rng.normal(0, 2, (8, V))
+    idx, v, lse = teacher(rng, z, 8, 1.0, tail)
+    other = [next(j for j in range(V) if j not in idx[r]) for r in range(8)]
+    z[1, idx[1, 2]] = z[2, other[2]] = math.nan
+    z[4, idx[4, 0]] = z[6, other[6]] = math.inf
+    loss, grad = TK.distill_loss_grad(ctx, torch.as_tensor(z, dtype=torch.float32).to(DT[dtype]).cuda(), cuda(idx.astype(np.int32)), cuda(v.astype(np.float32)),
+                                      None if lse is None else cuda(lse.astype(np.float32)))
+    for r in range(8):
+        if r in (1, 2, 4, 6):
+            assert loss[r].isnan() and grad[r].isnan().all(), r
+        else:
+            assert loss[r].isfinite() and grad[r].isfinite().all(), r
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [18, 5001, 140001])
+def test_distill_in_place_equals_out_of_place(ctx, V, dtype, tail):
+    """The gradient over the logits themselves, rows of masks' lowest values (read a second time) and of weight 0 among them."""
+    rng = np.random.default_rng(V)
+    z = rng.normal(0, 2, (6, V))
+    idx, v, lse = teacher(rng, z, 4, 1.0, tail)
+    z[1] = np.where(rng.random(V) < 0.7, -3e38, z[1])
+    z[2] = -3e38
+    z[2, idx[2]] = -1e38
+    z[3] = -3e38
+    z[4, 1] = -math.inf
+    w = np.array([1, 2, 0.5, 1, 1, 0])
+    t = torch.as_tensor(z, dtype=torch.float32).to(DT[dtype]).cuda()
+    args = [cuda(idx.astype(np.int32)), cuda(v.astype(np.float32)), None if lse is None else cuda(lse.astype(np.float32)), cuda(w.astype(np.float32))]
+    loss, grad = TK.distill_loss_grad(ctx, t, *args)
+    assert grad.isfinite().all()
+    over, same = TK.distill_loss_grad(ctx, t, *args, in_place=True)
+    assert same.data_ptr() == t.data_ptr() and torch.equal(over, loss) and torch.equal(same, grad)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("V, times", [(30, 1), (300, 1), (9000, 1), (9000, 130)])
+def test_verify_poisoned_rows_of_16_bits(ctx, V, times, dtype):
+    """NaN and +inf in target and draft rows, and rows of nothing: rejected, drawn from p or -1."""
+    rng = np.random.default_rng(V)
+    B, K = 10, 3
+    base = rng.normal(0, 2, (B, K + 1, V))
+    p = torch.as_tensor(base, dtype=torch.float32).to(DT[dtype])
+    q = p[:, :K].clone()
+    x = rng.integers(0, V, (B, K)).astype(np.int32)
+    ua, us = rng.random((B, K), dtype=np.float32) * np.float32(0.5), rng.random(B, dtype=np.float32)
+    p[0, 0, 0] = p[1, 1, V - 1] = p[2, 3, V // 2] = math.nan
+    p[3, 0, 1] = p[4, 2, V - 1] = p[5, 3, 0] = math.inf
+    q[6, 0, V - 1] = math.nan
+    q[7, 1, 2] = math.inf
+    q[8, 2] = -math.inf
+    p[9, 1] = -math.inf
+    tp, tq = p.cuda().repeat(times, 1, 1), q.cuda().repeat(times, 1, 1)
+    tx, tua, tus = repeated((x, ua, us), times)
+    for draft in (tq, None):
+        tok, acc, _ = (t.view(times, B, *t.shape[1:]).cpu().numpy() for t in TK.verify_drafts(ctx, tp, tx, tua, tus, draft_logits=draft))
+        for b in range(B):
+            want, a, _, margin = R.verify(p[b].double().numpy(), None if draft is None else q[b].double().numpy(), x[b], K, ua[b], us[b], 1.0)
+            assert margin > 1e-5
+            assert (tok[:, b] == want).all() and (acc[:, b] == a).all(), (b, tok[0, b], want)
