@@ -261,7 +261,10 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
       for (int k = tid; k < K; k += 64) { st[k] *= inv; slt[k] -= ls; }
       sum = 1.0;
     }
-    if (tid == 0) { steacher[0] = sum; steacher[1] = TAIL ? (sum > 1.0 ? 0.0 : 1.0 - sum) : 0.0; }
+    bool filled = false;                     // (a teacher without a slot has no tail either)
+    if constexpr (TAIL) for (int k = tid; k < K; k += 64) filled |= ssame[k] != 0;
+    filled = __any(filled);
+    if (tid == 0) { steacher[0] = sum; steacher[1] = TAIL && filled ? (sum > 1.0 ? 0.0 : 1.0 - sum) : 0.0; }
     if constexpr (TAIL) {
       float zm = -INFINITY;
       for (int k = tid; k < K; k += 64) if (ssame[k]) zm = fmaxf(zm, sz[k]);
@@ -335,7 +338,7 @@ __global__ __launch_bounds__(T) void distill_kernel(DistillArgs a) {
     S = ms.s * (double)tk_exp2((ms.m - B) * a.c) + stop.s * (double)tk_exp2((stop.m - B) * a.c);
     tT = ms.m == -INFINITY ? 0.0 : steacher[1];   // no logit outside top: the tail is left out
   }
-  if (S == 0.0 || (!TAIL && sumT == 0.0)) return zeros();   // nothing in the student's row, or nothing in the teacher's (the same for every thread)
+  if (S == 0.0 || (sumT == 0.0 && steacher[1] == 0.0)) return zeros();   // nothing in the student's row, or nothing in the teacher's (the same for every thread)
   if (tid < 64) {
     // With a tail, an error of s_T that is in the whole's sum too meets s_T - t_T only; one of the factor that takes it there meets 1: that factor in fp64.
     const double whole = TAIL ? ms.s * exp2(((double)ms.m - (double)tk_base(M)) * (double)a.c) + stop.s * exp2(((double)stop.m - (double)tk_base(M)) * (double)a.c) : S;

@@ -222,3 +222,19 @@ def test_verify_poisoned_rows_of_16_bits(ctx, V, times, dtype):
             want, a, _, margin = R.verify(p[b].double().numpy(), None if draft is None else q[b].double().numpy(), x[b], K, ua[b], us[b], 1.0)
             assert margin > 1e-5
             assert (tok[:, b] == want).all() and (acc[:, b] == a).all(), (b, tok[0, b], want)
+
+
+# ------------------------------------------------------------------------------------------ rows without a teacher
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V", [40, 5001, 140001])
+def test_distill_rows_without_a_filled_slot(ctx, V, tail):
+    """Loss and gradient are 0 whatever the row holds, a NaN or +inf among it."""
+    rng = np.random.default_rng(V)
+    z = rng.normal(0, 2, (5, V)).astype(np.float32)
+    z[1, V // 2], z[2, 0] = math.nan, math.inf
+    idx = np.full((5, 6), -1, np.int32)
+    idx[3] = V
+    idx[4, 2] = 3                              # a row that has one
+    v = rng.normal(0, 1, (5, 6)).astype(np.float32)
+    loss, grad = TK.distill_loss_grad(ctx, cuda(z), cuda(idx), cuda(v), cuda(np.float32([1, 1, -math.inf, 2, 3])) if tail else None)
+    assert (loss[:4] == 0).all() and (grad[:4] == 0).all() and loss[4] > 0 and (grad[4] != 0).any()
