@@ -1020,7 +1020,7 @@ template <int DT, int HOW> __device__ int vf_accept(const VerifyArgs& a, int b, 
     const bool ok = decide(srow[tid], a.draft ? srow[heads + tid] : srow[tid], &p, &uq);
     if constexpr (HOW == VF_STATS) sstate[tid] = fabs(uq - p) < a.close * fmax(uq, p) ? VF_CLOSE : (ok ? VF_YES : VF_NO);
     if (!ok || (HOW == VF_STATS && sstate[tid] == VF_CLOSE)) atomicMin(sat, tid);
-    else if (write) logp = vf_logp(a, srow[tid], zp);
+    else if (HOW != VF_STATS && write) logp = vf_logp(a, srow[tid], zp);   // (before the barrier: it is on the way to the token there)
   }
   __syncthreads();
   int at = *sat;
@@ -1031,7 +1031,7 @@ template <int DT, int HOW> __device__ int vf_accept(const VerifyArgs& a, int b, 
       if (tid == at) {
         double p, uq;
         sstate[at] = decide(ps, qs, &p, &uq) ? VF_YES : VF_NO;
-        logp = vf_logp(a, ps, zp);
+        srow[at] = ps;
       }
       __syncthreads();
       while (at < n && sstate[at] == VF_YES) ++at;
@@ -1039,6 +1039,7 @@ template <int DT, int HOW> __device__ int vf_accept(const VerifyArgs& a, int b, 
     }
   }
   if (write) {
+    if (HOW == VF_STATS && tid < at) logp = vf_logp(a, srow[tid], zp);
     if (tid < at) { a.out[t0 + tid] = x; if (a.logprobs) a.logprobs[t0 + tid] = (float)logp; }
     else if (tid > at && tid <= a.K) { a.out[t0 + tid] = -1; if (a.logprobs) a.logprobs[t0 + tid] = 0.0f; }
     if (tid == 0) a.accepted[b] = at;
@@ -1125,7 +1126,7 @@ template <int DT> struct VfWeight {
   double np, nq, none;
   int V, skip;
   __device__ __forceinline__ VfWeight(const VerifyArgs& a, const double* table, const char* prow, const VfSum& ps, const char* qrow, const VfSum& qs)
-    : prow(prow), qrow(qrow), ep{table, 32.0 * vf_slope(a, ps.e), 32.0 * ps.e}, eq{table, 32.0 * vf_slope(a, qs.e), 32.0 * qs.e}, np(1.0 / ps.s), nq((1.0 + VF_SAME) / qs.s),
+    : prow(prow), qrow(qrow), ep{table, 32.0 * vf_slope(a, ps.e), 32.0 * ps.e}, eq{table, 32.0 * vf_slope(a, qs.e), 32.0 * qs.e}, np(1.0 / ps.s), nq(1.0 / qs.s * (1.0 + VF_SAME)),
       none(2.0 * VF_NOTHING * np), V(a.V), skip(-1) {}
   __device__ __forceinline__ void leave_out(int token) { if ((uint32_t)token < (uint32_t)V) skip = token; }   // a looked-up token that was rejected
   __device__ __forceinline__ bool less() const { return qrow || skip >= 0; }
