@@ -3,15 +3,15 @@
 //   cbm_distill_loss_grad  distillation from a teacher's top logits: loss and gradient in one call, as cbm_ppo_loss_grad / cbm_impala_loss_grad
 //   cbm_verify_drafts      drafted tokens against the target's probabilities (the truncated ratio of cbm_vtrace, per token), and the next token
 // All are bound by reading the logits once (the gradient: and writing it once).  Rows start at any element (odd vocabularies): 16-byte loads
-// at element alignment, which the load unit takes.  Row statistics are (maximum, sum) pairs: sums of up to a few hundred terms a thread in
-// fp32, everything across threads and everything that a decision or a loss depends on in fp64.
+// at element alignment, which the load unit takes.  Row statistics are (maximum, sum) pairs: a thread's terms in fp32 (steps of at most 64, up to 2048 in all
+// at 2^19 tokens), everything across threads and everything that a decision or a loss depends on in fp64.
 #include "cbm_ctx.h"
 #include <float.h>
 #include <math.h>
 
 namespace {
 
-constexpr int TK_MAX_VOCAB = 1 << 19;   // indices are 19 bits of a key in the top-K kernels; a row's bitmap (one bit a token) fits 64 KB of LDS
+constexpr int TK_MAX_VOCAB = 1 << 19;   // indices are 19 bits of a key in the top-K kernels; a row's bitmap (one bit a token and a word) is 64 KB of the 160 KB LDS
 constexpr int TK_MAX_TOP = 256;         // slots of a row: four a lane of the wave that owns the row's teacher
 constexpr int TK_MAX_DRAFTS = 128;      // one thread a draft in the acceptance step
 constexpr int TK_MAX_ROWS = 1 << 22;    // a launch holds fewer than 2^32 threads, a row up to 1024
@@ -147,9 +147,10 @@ template <int T> __device__ __forceinline__ MS block_lse(float m, float s, float
 // maximum of its own, not a difference that cancels, and the top tokens join it from the wave that holds the teacher.  Every other token's gradient is
 // one coefficient times an exponential; the top tokens' gradients are stored last, over what the stream left.
 // log2(e) / tau is rounded to fp32 once and used so throughout the student's side, loss included: the loss of a temperature off by 6e-8.
-// Bound by memory where there are rows enough: 3840 rows of 131072 bf16, K 64, 427 us = 4.7 TB/s of one reading and one writing (a large copy reaches 4.85);
-// 777 rows of 50021 fp32 with a tail 66 us = 4.2 TB/s (three rows a compute unit, and a bit: the last ones are alone).  Small calls are bound by the
-// launch: 3840 rows of 18 actions take 10 us, 60 rows of 32768 9 us.  One pass over the row in memory costs a block's own latency (load, statistics,
+// Bound by memory where there are rows enough: 3840 rows of 131072 bf16, K 64, 427 us = 4.7 TB/s of one reading and one writing (a large copy reaches 4.85),
+// the loss alone 217 us = 4.6 TB/s; 777 rows of 50021 fp32 with a tail, a fifth of them padding that is written only, 71 us = 3.9 TB/s (three rows a compute
+// unit, and a bit: the last ones are alone).  Small calls are bound by the launch: 3840 rows of 18 actions take 10.6 us, 60 rows of 32768 8.6.  A few rows
+// are bound by one block's latency: 1 row of 131072 bf16 18 us, 64 rows 20.  One pass over the row in memory costs a block's own latency (load, statistics,
 // barrier, gradient), which the other blocks of a compute unit cover; keeping the next row's loads in flight in the same block needed the registers of a
 // second row and was slower (spills).
 struct DistillArgs {
@@ -403,7 +404,7 @@ void distill_launch(const DistillArgs& a, hipStream_t st) {
 // 8 vectors a thread stay (80 registers); 6 blocks of 256 threads share a compute unit, 3 of 512, and one of 1024 is alone there: the loads, sums and stores of
 // neighbours overlap.  A larger block reads less of its row twice, a smaller one has more company.  3840 rows with gradient, us by blocks of 256 / 512 / 1024:
 // 20000 bf16 (2500 vectors) 70 / 86 / 144, 32768 bf16 122 / 106 / 170, 65536 bf16 (8192) 260 / 216 / 251, 50021 fp32 (12506) 453 / 358 / 325,
-// 131072 bf16 (16384) 575 / 470 / 427.  12 or 16 vectors a thread: 424 and 442 there, 320 and 318 at 50021 fp32.  K <= T.
+// 131072 bf16 (16384) 575 / 470 / 427.  (Fewer rows go by the same rule.)  12 or 16 vectors a thread: 424 and 442 there, 320 and 318 at 50021 fp32.  K <= T.
 template <int DT>
 void distill_dispatch(const DistillArgs& a, hipStream_t st) {
   const int nv = (a.V + Lg<DT>::VEC - 1) / Lg<DT>::VEC;
@@ -424,9 +425,11 @@ void distill_dispatch(const DistillArgs& a, hipStream_t st) {
 // K-th largest key of the buffer raises it, so that a row of n chunks appends about K (1 + log2 n) keys.  An element that only equals the bar comes
 // behind K others and is left out.  Should the buffer overflow all the same (rising rows), the lanes that found no room wait while it is cut to T keys,
 // and a chunk that alone would fill it is held to the exact K-th of its threads' maxima: K threads, EPT K keys, the room there is.
-// 3840 rows of 32768 bf16, K 32: 62 us = 4.1 TB/s, 1009 of 100003 fp16 at odd addresses, K 128: 64 us = 3.2 TB/s.  Long rows are bound by what an element
-// costs beside its load (maximum, exponential, comparison with the bar: 7 instructions); short ones with large K by the buffer: choosing the bar and
-// ordering K keys (each counts those above it, n^2 / 64 comparisons a block).  16384 rows of 1000: K 8 20 us, K 64 46, K 256 379.
+// 3840 rows of 32768 bf16, K 32: 66 us = 3.8 TB/s, 1009 of 100003 fp16 at odd addresses, K 128: 65 us = 3.1 TB/s.  Counted there: 13.7 and 13.4 vector
+// instructions an element (it is decoded for the maximum and for the sum), the vector units busy for 67 and 51 % of the time: 16-bit rows are bound by them and
+// by the barriers of a block (first bar, cuts, order), which with K 128 have 14.6 waves a compute unit to hide behind.  Short rows with large K are bound by
+// the buffer: choosing the bar and ordering K keys (each counts those above it, n^2 / 64 comparisons a block).  16384 rows of 1000: K 8 20 us, K 64 46,
+// K 256 364 (vector units busy for 60 % of it, LDS for 56).
 struct TopArgs {
   const char* logits; int64_t ld;
   int32_t* idx; float* val; float* lse;
@@ -741,8 +744,8 @@ TopPlan top_plan(int rows, int V, int K) {
   // K = 128, by 512 threads 299 us, by 256 221; 131072 bf16, K = 256, by 1024 558, by 512 372; fp32 and smaller K the same
   p.threads = K <= 32 && V <= 1024 ? 64 : (K <= 64 && V <= 2048 ? 128 : (K <= 128 ? 256 : 512));
   // Few rows leave compute units empty: up to 128 long ones are split until there are about 512 blocks, and joined (a second kernel); up to 255 others go to
-  // wider blocks.  us split / not: 60 x 32768 bf16, K = 32, 20 / 15; 1 x 131072 bf16, K = 64, 21 / 30; 60 of them 21 / 31, 200 34 / 34; 1 x 100003 fp16, K = 128, 27 / 31,
-  // 200 39 / 36; K = 256 (by 512 threads either way) 1 x 131072 38 / 40, 60 58 / 40.
+  // wider blocks.  The border of 49152 tokens lies between the measured 32768 and 100003.  us split / not: 60 x 32768 bf16, K = 32, 20 / 15;
+  // 1 x 131072 bf16, K = 64, 21 / 30; 60 of them 21 / 31, 200 34 / 34; 1 x 100003 fp16, K = 128, 27 / 31, 200 39 / 36; K = 256 (by 512 threads either way) 1 x 131072 38 / 40, 60 58 / 40.
   const bool split = rows <= 128 && V > 49152 && p.threads == TOP_SPLIT_T;   // (K <= 128)
   if (!split && rows < 256 && V > 16384) p.threads = 512;
   p.cap = top_ept(p.threads, V) * K + p.threads;
@@ -794,9 +797,11 @@ template <int DT> void top_dispatch(const TopArgs& a, const TopPlan& p, hipStrea
 //   verify_stats_kernel           (maximum, sum) in fp32 of the drafted positions' rows
 //   verify_sums_kernel<VF_STATS>  acceptance, and the fp64 sums of the one or two rows that the token is drawn from
 //   verify_pick_kernel<VF_STATS>  the rest as above
-// Bound: at 64 sequences of up to 8 drafts, 131072 bf16, 80 us: statistics 29 (220 MB at most, rows behind n_draft unread: exponentials and loads alike), sums 21
-// and pick 29 (17 and 34 MB: 20 fp64 instructions an exponential, at half rate, and the chain acceptance, chunk sums, last block, scan, token).  One sequence
-// of 4 drafts: sums 6, pick 15 (that chain alone).  37 sequences of 5 looked-up drafts, 50021 fp16: 13 and 15.  120 sequences of 7, 18 actions: one kernel, 8.
+// Bound: at 64 sequences of up to 8 drafts, 131072 bf16, 79 us a call.  Statistics 29 (134 MB where lengths are 4 in the mean, 268 at most; rows behind n_draft are
+// unread): 4.6 TB/s.  Sums 23 and pick 29 (17 MB of target rows, and as much of draft rows where all end in a rejection): an fp64 exponential is 20 instructions, fp64 at the rate of
+// unpacked fp32, which keeps the vector units busy for 44 and 20 % of the time; the rest is the chain acceptance, chunk sums, last block, scan, token, with a
+// chunk or two a wave behind it.  One sequence of 4 drafts: sums 6, pick 14 to 18 (that chain alone).  37 sequences of 5 looked-up drafts, 50021 fp16:
+// 13 and 15.  120 sequences of 7, 18 actions: one kernel, 9.  No drafts, 131072 bf16: one sequence 6 + 15, 64 11 + 14.  Greedy, 64 sequences of up to 8: 23 + 6.
 constexpr int VF_T = 256, VF_WAVES = VF_T / 64, VF_CHUNK = 2048;   // 32 tokens a lane: what a chunk costs beside its exps (reductions) is shared by that many
 enum { VF_STATS, VF_SUMS, VF_ONE };          // three kernels, two, one
 struct VfSum { double e, s; };               // s 2^e; nothing: s = 0, e = -inf; a NaN among the logits: s NaN; +inf: e = +inf
@@ -1286,7 +1291,7 @@ __global__ __launch_bounds__(VF_T) void verify_pick_kernel(VerifyArgs a) {
 }
 
 // Rows of one chunk and few of them: a block a sequence.  Up to 16 lanes' vectors: 16 rows at once, else a wave a row.  The weights of the row that is
-// drawn from are looked at once.
+// drawn from are looked at once.  Held to 128 registers (4 waves a SIMD), at which 34 (fp32) or 4 (16 bits) are spilled to scratch, 140 and 20 bytes a lane.
 template <int DT>
 __global__ __launch_bounds__(VF_T, 4) void verify_one_kernel(VerifyArgs a) {
   constexpr int VEC = Lg<DT>::VEC, U = VF_CHUNK / 64 / VEC;

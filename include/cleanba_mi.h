@@ -306,13 +306,18 @@ int64_t cbm_top_logits_workspace(int32_t dtype, int32_t rows, int32_t vocab, int
 int cbm_top_logits(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, int32_t k, double temperature,
                    int32_t* idx, float* values, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 /* Distillation from a teacher's top logits: KL(teacher || student) tau^2 per row times row_weight (NULL: 1), and its gradient.
- *  teacher_idx i32 [rows][k], teacher_logits f32 [rows][k] (k 1..256): the teacher's slots; an index outside [0, vocab) is an empty slot, a token in
- *    several slots has their probabilities added.
+ *  teacher_idx i32 [rows][k], teacher_logits f32 [rows][k] (k 1..256): the teacher's slots; an index outside [0, vocab) is an empty slot.
  *  teacher_lse f32 [rows] or NULL.  NULL: the teacher is softmax over the slots.  Given (at the same tau): slot probabilities are
  *    exp(logit / tau - lse), what they leave of 1 is one more class, "any other token", in teacher and student alike.
+ *  With t the teacher's and s the student's probabilities and T the class of other tokens (teacher_lse alone), w the weight,
+ *    loss = w tau^2 [sum over slots t_k (log t_k - log s_{i_k}) + t_T (log t_T - log s_T)],
+ *    dlogits_j = w tau [s_j (sum t_k + t_T) - (sum of t_k over the slots of token j) - (j in T) t_T s_j / s_T].
+ *    A token in several slots has their probabilities added; the loss, a sum over slots, is then less than the KL by that probability times the entropy of
+ *    its split, whatever the student.
  *  loss f32 [rows]; dlogits: like logits, rows grad_stride apart, or NULL for the loss alone; it may be logits itself (same pointer and stride).
  * Loss and gradient of a row are 0 where its weight is 0 (the row is not read), where all its logits are -inf, and where the teacher has no filled slot.
- * The class of other tokens is left out where the student has no logit above -inf for it.  A student's -inf on a token of the teacher gives loss +inf. */
+ * The class of other tokens is left out where the student has no logit above -inf for it.  A student's -inf on a token of the teacher gives loss +inf.
+ * In other rows a NaN or +inf among the logits makes loss and gradient of its row NaN. */
 int cbm_distill_loss_grad(cbm_ctx* ctx, const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t row_stride, const int32_t* teacher_idx,
                           const float* teacher_logits, int32_t k, const float* teacher_lse, const float* row_weight, double temperature, float* loss,
                           void* dlogits, int64_t grad_stride, void* stream);
@@ -326,6 +331,7 @@ int cbm_distill_loss_grad(cbm_ctx* ctx, const void* logits, int32_t dtype, int32
  *  tokens i32 [batch][drafts+1]: the accepted ones, the drawn one, then -1; accepted i32 [batch]; logprobs f32 [batch][drafts+1] or NULL: log p of each
  *    token, 0 behind the last.  temperature 0: p is one-hot at the largest logit (lowest index of equal ones), random numbers and draft_logits are not
  *    looked at and may be NULL, logprobs are 0.
+ *  A probability under about 2^-990 of the row's largest counts as 0 (such a token is neither accepted nor drawn, not by a random number of 0 either).
  *  A token outside [0, vocab) is rejected; so is one whose draft row is no distribution (only -inf, a NaN or +inf), and then the token is drawn from p.
  *  A target row that is no distribution rejects, and the drawn token is -1.  drafts = 0 samples one token a sequence. */
 int64_t cbm_verify_drafts_workspace(int32_t dtype, int32_t batch, int32_t drafts, int32_t vocab, int32_t with_draft_logits, double temperature);
