@@ -745,7 +745,8 @@ TopPlan top_plan(int rows, int V, int K) {
   p.threads = K <= 32 && V <= 1024 ? 64 : (K <= 64 && V <= 2048 ? 128 : (K <= 128 ? 256 : 512));
   // Few rows leave compute units empty: up to 128 long ones are split until there are about 512 blocks, and joined (a second kernel); up to 255 others go to
   // wider blocks.  The border of 49152 tokens lies between the measured 32768 and 100003.  us split / not: 60 x 32768 bf16, K = 32, 20 / 15;
-  // 1 x 131072 bf16, K = 64, 21 / 30; 60 of them 21 / 31, 200 34 / 34; 1 x 100003 fp16, K = 128, 27 / 31, 200 39 / 36; K = 256 (by 512 threads either way) 1 x 131072 38 / 40, 60 58 / 40.
+  // 1 x 131072 bf16, K = 64, 21 / 30; 60 of them 21 / 31, 200 34 / 34; 1 x 100003 fp16, K = 128, 27 / 31, 200 39 / 36; K = 256
+  // (by 512 threads either way) 1 x 131072 38 / 40, 60 58 / 40.
   const bool split = rows <= 128 && V > 49152 && p.threads == TOP_SPLIT_T;   // (K <= 128)
   if (!split && rows < 256 && V > 16384) p.threads = 512;
   p.cap = top_ept(p.threads, V) * K + p.threads;
